@@ -288,6 +288,41 @@ int dsa_v4_attention(const void* q, const void* ori_kv, const void* cmp_kv, cons
                      float* lse, int32_t T, int32_t H, int32_t width, int32_t ori_pool_rows, int32_t cmp_pool_rows,
                      float sm_scale, int32_t dtype, int32_t nsplit, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Queries or keys of dsa_norm_rope: x [B, S, heads, D] with unit inner stride (strides in elements).  norm: 0 none, 1 RMS, 2 layer;
+ * weight and bias [norm_dim] or NULL, fp32 when params_fp32, else the rows' type.  Output dims [0, split) go to y, the rest to
+ * y_tail (split = D: all to y): row (b * S + s) * heads + h, or with slots [B * S] (int32, int64 when slots_int64) row
+ * slots[b * S + s] * heads + h of the y_slots * heads rows of a cache; a slot outside [0, y_slots) is not written. */
+typedef struct dsa_rope_rows {
+  const void* x;
+  int64_t stride_b, stride_s, stride_h;
+  int32_t heads, norm;
+  const void* weight;
+  const void* bias;
+  int32_t params_fp32, split;
+  void* y;
+  void* y_tail;
+  const void* slots;
+  int64_t y_slots;
+  int32_t slots_int64, reserved;
+} dsa_rope_rows;
+
+/* Norm of the leading norm_dim dims of every head's row, then rotation of its dims [rope_start, rope_start + rope_dim) by
+ * positions[b * S + s] * inv_freq[i] (cos and sin times rope_scale): pairs (2i, 2i + 1) when interleaved, else (i, i + rope_dim / 2).
+ * positions [B * S] int32 or int64, inv_freq [rope_dim / 2] fp32.  q or k may be NULL.  One launch.  No reference counterpart: the
+ * reference's attention and indexer examples take rotated queries and keys as inputs. */
+int dsa_norm_rope(const dsa_rope_rows* q, const dsa_rope_rows* k, const void* positions, int32_t positions_int64, const float* inv_freq,
+                  int32_t B, int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved,
+                  float rope_scale, float eps, int32_t dtype, void* stream);
+
+/* Gradients of one side: rows->x (read with a norm only), rows->y = dx [B, S, heads, D] contiguous; dy with unit inner stride.
+ * d_weight / d_bias [norm_dim] (the parameters' type) or NULL; when one is given, workspace holds at least
+ * dsa_norm_rope_bwd_workspace_bytes(norm_dim) bytes.  Sums are taken in a fixed order. */
+size_t dsa_norm_rope_bwd_workspace_bytes(int32_t norm_dim);
+int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stride_b, int64_t dy_stride_s, int64_t dy_stride_h,
+                      const void* positions, int32_t positions_int64, const float* inv_freq, int32_t B, int32_t S, int32_t D,
+                      int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps,
+                      void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

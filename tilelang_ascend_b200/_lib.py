@@ -15,6 +15,15 @@ LIB_PATH = os.path.join(_PKG, "libdsa_b200.so")
 DTYPE_BF16, DTYPE_FP16 = 0, 1
 IMPL_AUTO, IMPL_GENERIC, IMPL_TENSOR_CORE = 0, 1, 2
 
+
+
+class RopeRows(ctypes.Structure):
+    """``dsa_rope_rows`` of the C header."""
+    _fields_ = [("x", c_void_p), ("stride_b", c_int64), ("stride_s", c_int64), ("stride_h", c_int64), ("heads", c_int32), ("norm", c_int32),
+                ("weight", c_void_p), ("bias", c_void_p), ("params_fp32", c_int32), ("split", c_int32), ("y", c_void_p), ("y_tail", c_void_p),
+                ("slots", c_void_p), ("y_slots", c_int64), ("slots_int64", c_int32), ("reserved", c_int32)]
+
+
 # name -> (restype, argtypes); must list every symbol include/dsa_b200.h declares
 SIGNATURES = {
     "dsa_init": (c_int32, []),
@@ -73,6 +82,11 @@ SIGNATURES = {
                                         c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32,
                                         c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                         c_void_p, c_size_t, c_int32, c_void_p]),
+    "dsa_norm_rope": (c_int32, [ctypes.POINTER(RopeRows), ctypes.POINTER(RopeRows), c_void_p, c_int32, c_void_p] + [c_int32] * 7
+                      + [c_float, c_float, c_int32, c_void_p]),
+    "dsa_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int32]),
+    "dsa_norm_rope_bwd": (c_int32, [ctypes.POINTER(RopeRows), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p] + [c_int32] * 7
+                          + [c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_int32, c_void_p]),
 }
 
 _lib = None

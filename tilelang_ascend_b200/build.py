@@ -17,9 +17,11 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 LIB = os.path.join(PKG, "libdsa_b200.so")
-SOURCES = ["capi.cu", "sparse_mla_fwd.cu", "sparse_mla_fwd_pair.cu", "sparse_mla_fwd_narrow.cu", "sparse_mla_bwd.cu", "sparse_mla_bwd_tc.cu", "indexer.cu", "topk.cu", "no_alloc.cu", "sink_combine.cu", "block_sparse_logits.cu", "selftest.cu"]
+SOURCES = ["capi.cu", "sparse_mla_fwd.cu", "sparse_mla_fwd_pair.cu", "sparse_mla_fwd_narrow.cu", "sparse_mla_bwd.cu", "sparse_mla_bwd_tc.cu", "indexer.cu", "topk.cu", "no_alloc.cu", "sink_combine.cu", "block_sparse_logits.cu", "selftest.cu", "norm_rope.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
+# sources whose results are held to fp32 (logarithms, sines): exact divisions, square roots and math functions
+PRECISE_SOURCES = {"norm_rope.cu"}
 
 
 def _nvcc() -> str:
@@ -48,7 +50,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
         path = os.path.join(CSRC, src)
         if force or _newer_than(obj, [path] + headers):
-            cmd = [nvcc, *NVCC_FLAGS, "-c", path, "-o", obj]
+            flags = [f for f in NVCC_FLAGS if f != "--use_fast_math" or src not in PRECISE_SOURCES]
+            cmd = [nvcc, *flags, "-c", path, "-o", obj]
             res = subprocess.run(cmd, capture_output=True, text=True)
             logs[src] = res.stdout + res.stderr
             if res.returncode != 0:

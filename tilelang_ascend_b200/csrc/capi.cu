@@ -8,6 +8,7 @@
 
 #include "../../include/dsa_b200.h"
 #include "launch_util.h"
+#include "norm_rope.h"
 #include "params.h"
 
 namespace dsa {
@@ -118,6 +119,39 @@ int fill_fwd_params(dsa::FwdParams* p, const void* q, const void* kv, const int3
   p->trace = g_trace;
 #endif
   return get_status_word(&p->status);
+}
+
+// One side of a norm + rotation call; fails on what the kernels do not handle.
+int fill_rope_side(dsa::RopeSide* sd, const dsa_rope_rows* r, int32_t D, int32_t norm_dim) {
+  *sd = dsa::RopeSide{};
+  sd->split = D;
+  if (!r) return 0;
+  if (!r->x && r->norm) return fail("null tensor pointer");
+  if (!r->y || (r->split < D && !r->y_tail)) return fail("null output pointer");
+  if (r->heads <= 0) return fail("heads must be positive");
+  if (r->norm < 0 || r->norm > 2) return fail("norm must be 0 (none), 1 (RMS) or 2 (layer)");
+  if (r->norm && norm_dim <= 0) return fail("a norm needs a positive norm_dim");
+  if (r->split <= 0 || r->split > D) return fail("split must be in [1, D]");
+  if (r->slots && r->y_slots < 0) return fail("y_slots must not be negative");
+  sd->x = dsa::RowView{r->x, r->stride_b, r->stride_s, r->stride_h};
+  sd->H = r->heads; sd->norm = r->norm; sd->weight = r->weight; sd->bias = r->bias; sd->param_fp32 = r->params_fp32;
+  sd->y = r->y; sd->y_tail = r->y_tail; sd->split = r->split; sd->slots = r->slots; sd->slots64 = r->slots_int64; sd->y_slots = r->y_slots;
+  return 0;
+}
+
+int fill_norm_rope(dsa::NormRopeParams* p, const void* positions, int32_t positions_int64, const float* inv_freq, int32_t B, int32_t S, int32_t D,
+                   int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps, int32_t dtype) {
+  if (!positions || !inv_freq) return fail("null tensor pointer");
+  if (!dtype_ok(dtype)) return fail("dtype must be 0 (bfloat16) or 1 (float16)");
+  if (B <= 0 || S <= 0 || D <= 0) return fail("B, S and D must be positive");
+  if (static_cast<int64_t>(B) * S > 0x3fffffffLL) return fail("B * S too large");
+  if (rope_dim <= 0 || rope_dim % 2 || rope_start < 0 || rope_dim > D || rope_start > D - rope_dim) return fail("the rotated dims must be an even number inside the row");
+  if (norm_dim < 0 || norm_dim > D) return fail("norm_dim must be in [0, D]");
+  if (!std::isfinite(rope_scale) || !std::isfinite(eps) || eps < 0.f) return fail("rope_scale must be finite, eps finite and not negative");
+  p->positions = positions; p->positions64 = positions_int64; p->inv_freq = inv_freq;
+  p->tokens = B * S; p->S = S; p->D = D; p->R = rope_dim; p->rope_start = rope_start; p->norm_dim = norm_dim; p->interleaved = interleaved ? 1 : 0;
+  p->rope_scale = rope_scale; p->eps = eps; p->inv_norm_dim = norm_dim ? 1.f / static_cast<float>(norm_dim) : 0.f;
+  return 0;
 }
 
 }  // namespace
@@ -531,6 +565,39 @@ int dsa_v4_build_joined_indices(const int32_t* cu_seqlens_q, const int32_t* sequ
                                                 cmp_pool_rows, B, T, S, tnd, ori_table_len, ori_block_size, ori_win_left, cmp_table_len, cmp_block_size,
                                                 cmp_ratio, scenario, K, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("v4_build_joined_indices launch", err) : 0;
+}
+
+int dsa_norm_rope(const dsa_rope_rows* q, const dsa_rope_rows* k, const void* positions, int32_t positions_int64, const float* inv_freq, int32_t B,
+                  int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps,
+                  int32_t dtype, void* stream) {
+  dsa::NormRopeParams p{};
+  if (!q && !k) return fail("queries or keys must be given");
+  if ((q && !q->x) || (k && !k->x)) return fail("null tensor pointer");
+  if (fill_norm_rope(&p, positions, positions_int64, inv_freq, B, S, D, rope_dim, rope_start, norm_dim, interleaved, rope_scale, eps, dtype)) return 1;
+  if (fill_rope_side(&p.side[0], q, D, norm_dim) || fill_rope_side(&p.side[1], k, D, norm_dim)) return 1;
+  int err = dsa::launch_norm_rope(p, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("norm_rope launch", err) : 0;
+}
+
+size_t dsa_norm_rope_bwd_workspace_bytes(int32_t norm_dim) { return norm_dim > 0 ? dsa::norm_rope_bwd_workspace_bytes(norm_dim) : 0; }
+
+int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stride_b, int64_t dy_stride_s, int64_t dy_stride_h, const void* positions,
+                      int32_t positions_int64, const float* inv_freq, int32_t B, int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start,
+                      int32_t norm_dim, int32_t interleaved, float rope_scale, float eps, void* d_weight, void* d_bias, void* workspace,
+                      size_t workspace_bytes, int32_t dtype, void* stream) {
+  dsa::NormRopeParams p{};
+  if (!rows || !dy) return fail("null tensor pointer");
+  if (fill_norm_rope(&p, positions, positions_int64, inv_freq, B, S, D, rope_dim, rope_start, norm_dim, interleaved, rope_scale, eps, dtype)) return 1;
+  if (fill_rope_side(&p.side[0], rows, D, norm_dim) || fill_rope_side(&p.side[1], nullptr, D, norm_dim)) return 1;
+  if (rows->slots || rows->split != D) return fail("the gradient is one contiguous tensor");
+  p.side[0].dy = dsa::RowView{dy, dy_stride_b, dy_stride_s, dy_stride_h};
+  if (d_weight || d_bias) {
+    if (!rows->norm) return fail("gradients of norm parameters need a norm");
+    if (!workspace || workspace_bytes < dsa::norm_rope_bwd_workspace_bytes(norm_dim)) return fail("workspace too small (see dsa_norm_rope_bwd_workspace_bytes)");
+    p.side[0].partials = static_cast<float*>(workspace);
+  }
+  int err = dsa::launch_norm_rope_bwd(p, d_weight, d_bias, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("norm_rope_bwd launch", err) : 0;
 }
 
 }  // extern "C"

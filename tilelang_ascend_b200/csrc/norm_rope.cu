@@ -1,0 +1,629 @@
+// Norm of every head's row and rotation by its token's position, in one pass (sm_100a).
+//
+//   y = rot(norm(x))      norm over the leading norm_dim dims (none, RMS, layer; weight and bias shared by the heads),
+//                         rotation of the dims [rope_start, rope_start + R), pairs (2i, 2i+1) or (i, i + R/2):
+//                         (a, b) -> (a cos - b sin, b cos + a sin), angle = position * inv_freq[i]
+//   backward: u = rot^T(dy); with n = (x - mean) rstd:  dweight = sum u n, dbias = sum u, g = u weight,
+//             dx = rstd (g - mean(g n) n [- mean(g)])
+//
+// Bound by memory: a row is read once and written once.  A group of 8, 16 or 32 lanes owns a row (16-byte units, all of them
+// in registers), a block owns a tile of tokens x heads; the cosines and sines of its tokens are made once per block, the
+// angle as an exact product reduced in 64 bits (a far position times a frequency has no fraction left in 32).
+// Everything is computed in fp32 and rounded once, on the store.
+//
+// Rows that do not come in 16-byte units (odd sizes, offsets or strides) take the *_any kernels: a warp per row, one element
+// at a time, the same arithmetic.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "launch_util.h"
+#include "norm_rope.h"
+
+namespace dsa {
+
+namespace nr {
+constexpr int kThreads = 256;
+constexpr int kMaxPairs = 2048;      // (token, pair) angles a block keeps: 16 KB
+constexpr int kMaxNormDim = 1024;    // widest row of the 16-byte kernels
+
+// cos and sin of position * inv_freq, times the rotation's scale.
+__device__ __forceinline__ float2 turn_of(long long position, float inv_freq, float scale) {
+  const double angle = static_cast<double>(position) * static_cast<double>(inv_freq);
+  const double turns = rint(angle * 0.15915494309189533577);          // 1 / 2 pi
+  double r = fma(-turns, 6.283185307179586232, angle);                // 2 pi in two parts
+  r = fma(-turns, 2.4492935982947064e-16, r);
+  float s, c;
+  sincosf(static_cast<float>(r), &s, &c);
+  return make_float2(c * scale, s * scale);
+}
+
+__device__ __forceinline__ long long position_of(const NormRopeParams& p, int token) {
+  return p.positions64 ? static_cast<const long long*>(p.positions)[token] : static_cast<const int*>(p.positions)[token];
+}
+
+// A norm's weight or bias: fp32, or the rows' own type.
+template <typename T>
+__device__ __forceinline__ float param_at(const void* w, int fp32, int i) {
+  return fp32 ? static_cast<const float*>(w)[i] : static_cast<float>(static_cast<const T*>(w)[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+  const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(e[j]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint4 w;
+  T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = static_cast<T>(v[j]);
+  return w;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// Address of element 0 of row (token, head) of a strided [B, S, H, D] tensor.
+template <typename T>
+__device__ __forceinline__ const T* row_of(const RowView& v, int S, int token, int head) {
+  const int b = token / S, s = token - b * S;
+  return static_cast<const T*>(v.base) + b * v.stride_b + s * v.stride_s + head * v.stride_h;
+}
+
+// Row number the output of (token, head) goes to, -1: it is not written.
+__device__ __forceinline__ long long out_row(const RopeSide& sd, int token, int head) {
+  if (!sd.slots) return static_cast<long long>(token) * sd.H + head;
+  const long long slot = sd.slots64 ? static_cast<const long long*>(sd.slots)[token] : static_cast<const int*>(sd.slots)[token];
+  return slot >= 0 && slot < sd.y_slots ? slot * sd.H + head : -1;
+}
+
+// The rotation of unit e0 .. e0 + 7 (dims relative to rope_start) of a row: v = this unit, o = its partner unit (halves only).
+// dir = +1 forward, -1 transposed.
+__device__ __forceinline__ void rotate8(float (&v)[8], const float (&o)[8], const float2* turns, int e0, int half, bool interleaved, float dir) {
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = turns[(e0 >> 1) + j];
+      const float a = v[2 * j], b = v[2 * j + 1], s = t.y * dir;
+      v[2 * j] = a * t.x - b * s;
+      v[2 * j + 1] = b * t.x + a * s;
+    }
+  } else {
+    const bool second = e0 >= half;
+    const int i0 = second ? e0 - half : e0;
+    const float sign = second ? dir : -dir;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 t = turns[i0 + j];
+      v[j] = v[j] * t.x + o[j] * (sign * t.y);
+    }
+  }
+}
+
+struct Tile {
+  int side, token0, head0, tokens, heads;
+};
+__device__ __forceinline__ Tile tile_of(const NormRopeParams& p, int block) {
+  Tile t;
+  t.side = block >= p.side[0].blocks;
+  const RopeSide& sd = p.side[t.side];
+  if (t.side) block -= p.side[0].blocks;
+  const int hb = (sd.H + sd.tile_heads - 1) / sd.tile_heads;
+  const int tb = block / hb;
+  t.token0 = tb * sd.tile_tokens;
+  t.head0 = (block - tb * hb) * sd.tile_heads;
+  t.tokens = min(sd.tile_tokens, p.tokens - t.token0);
+  t.heads = min(sd.tile_heads, sd.H - t.head0);
+  return t;
+}
+}  // namespace nr
+
+// -------------------------------------------------------------------------------------------------
+// forward, 16-byte units
+// -------------------------------------------------------------------------------------------------
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+  using namespace nr;
+  extern __shared__ float2 turns[];                       // [tile_tokens][R / 2]
+  __shared__ __align__(16) float sw[kMaxNormDim], sb[kMaxNormDim];
+  const Tile t = tile_of(p, blockIdx.x);
+  const RopeSide& sd = p.side[t.side];
+  const int tid = threadIdx.x, lane = tid % G, group = tid / G;
+  constexpr int kGroups = kThreads / G;
+  const int units = p.D >> 3, half = p.R >> 1, rows = t.tokens * t.heads;
+
+  uint4 raw[NV];
+  auto fetch = [&](int row) {
+    const T* x = row_of<T>(sd.x, p.S, t.token0 + row / t.heads, t.head0 + row % t.heads);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + G * i < units) raw[i] = ld_stream(x + (lane + G * i) * 8);
+  };
+  if (group < rows) fetch(group);   // the first row travels while the angles are made
+  for (int i = tid; i < t.tokens * half; i += kThreads) {
+    const int tk = i / half;
+    turns[i] = turn_of(position_of(p, t.token0 + tk), p.inv_freq[i - tk * half], p.rope_scale);
+  }
+  if (sd.norm)
+    for (int i = tid; i < p.norm_dim; i += kThreads) {
+      sw[i] = sd.weight ? param_at<T>(sd.weight, sd.param_fp32, i) : 1.f;
+      sb[i] = sd.bias ? param_at<T>(sd.bias, sd.param_fp32, i) : 0.f;
+    }
+  __syncthreads();
+
+  // (groups of one warp take the same number of turns through the loop, so that its shuffles see all lanes)
+  for (int row0 = 0; row0 < rows; row0 += kGroups) {
+    const int row = row0 + group;
+    const bool live = row < rows;
+    const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (live && lane + G * i < units) unpack8<T>(raw[i], v[i]);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+    }
+    if (row + kGroups < rows) fetch(row + kGroups);
+    float mean = 0.f, rstd = 1.f;
+    if (sd.norm) {
+      if (sd.norm == kNormLayer) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[i][j];
+          }
+        mean = group_sum<G>(s) * p.inv_norm_dim;
+      }
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) q += (v[i][j] - mean) * (v[i][j] - mean);
+        }
+      rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = (lane + G * i) * 8;
+        if (e < p.norm_dim) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - mean) * rstd * sw[e + j] + sb[e + j];
+        }
+      }
+    }
+    const long long orow = live ? out_row(sd, token, head) : -1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (lane + G * i) * 8, r = e - p.rope_start;
+      if (!live || e >= p.D) continue;
+      if (r >= 0 && r < p.R) {
+        float o[8];
+        if (!p.interleaved) {   // the pair's other members lie in another lane's unit: read them again (the row is in L2) and norm them
+          const int pe = r < half ? e + half : e - half;
+          unpack8<T>(__ldg(reinterpret_cast<const uint4*>(row_of<T>(sd.x, p.S, token, head) + pe)), o);
+          if (sd.norm && pe < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = (o[j] - mean) * rstd * sw[pe + j] + sb[pe + j];
+          }
+        }
+        rotate8(v[i], o, turns + tk * half, r, half, p.interleaved, 1.f);
+      }
+      if (orow >= 0) {
+        T* y = e < sd.split ? static_cast<T*>(sd.y) + orow * sd.split + e : static_cast<T*>(sd.y_tail) + orow * (p.D - sd.split) + (e - sd.split);
+        *reinterpret_cast<uint4*>(y) = pack8<T>(v[i]);
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------
+// backward of one side, 16-byte units.  With a norm every block leaves the sums of its rows for dweight and dbias in its own
+// line of the workspace (norm_rope_param_grad_kernel adds the lines up in a fixed order).
+// -------------------------------------------------------------------------------------------------
+template <typename T, int G, int NV, bool kNorm>
+__global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
+  using namespace nr;
+  extern __shared__ float2 turns[];
+  __shared__ __align__(16) float sw[kNorm ? kMaxNormDim : 1], sdw[kNorm ? kMaxNormDim : 1], sdb[kNorm ? kMaxNormDim : 1];
+  const RopeSide& sd = p.side[0];
+  const int tid = threadIdx.x, lane = tid % G, group = tid / G;
+  constexpr int kGroups = kThreads / G;
+  const int units = p.D >> 3, half = p.R >> 1;
+  float dw[kNorm ? NV : 1][8], db[kNorm ? NV : 1][8];
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f;
+    }
+    for (int i = tid; i < p.norm_dim; i += kThreads) {
+      sw[i] = sd.weight ? param_at<T>(sd.weight, sd.param_fp32, i) : 1.f;
+      sdw[i] = sdb[i] = 0.f;
+    }
+  }
+  for (int tile = blockIdx.x; tile < sd.blocks; tile += gridDim.x) {
+    const Tile t = tile_of(p, tile);
+    const int rows = t.tokens * t.heads;
+    __syncthreads();   // the last tile's angles have been used
+    for (int i = tid; i < t.tokens * half; i += kThreads) {
+      const int tk = i / half;
+      turns[i] = turn_of(position_of(p, t.token0 + tk), p.inv_freq[i - tk * half], p.rope_scale);
+    }
+    __syncthreads();
+    for (int row0 = 0; row0 < rows; row0 += kGroups) {
+      const int row = row0 + group;
+      const bool live = row < rows;
+      const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
+      const T* dy = row_of<T>(sd.dy, p.S, token, head);
+      float v[NV][8], x[kNorm ? NV : 1][8];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        uint4 w = make_uint4(0, 0, 0, 0), wx = w;
+        if (live && lane + G * i < units) {
+          w = ld_stream(dy + (lane + G * i) * 8);
+          if constexpr (kNorm)
+            if ((lane + G * i) * 8 < p.norm_dim) wx = ld_stream(row_of<T>(sd.x, p.S, token, head) + (lane + G * i) * 8);
+        }
+        unpack8<T>(w, v[i]);
+        if constexpr (kNorm) unpack8<T>(wx, x[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = (lane + G * i) * 8, r = e - p.rope_start;
+        if (live && e < p.D && r >= 0 && r < p.R) {
+          float o[8];
+          if (!p.interleaved) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(dy + (r < half ? e + half : e - half))), o);
+          rotate8(v[i], o, turns + tk * half, r, half, p.interleaved, -1.f);
+        }
+      }
+      if constexpr (kNorm) {
+        float mean = 0.f;
+        if (sd.norm == kNormLayer) {
+          float s = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += x[i][j];   // (units beyond norm_dim hold zeros)
+          }
+          mean = group_sum<G>(s) * p.inv_norm_dim;
+        }
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { x[i][j] -= mean; q += x[i][j] * x[i][j]; }
+          }
+        const float rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
+        float gn = 0.f, gs = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int e = (lane + G * i) * 8;
+          if (e < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              x[i][j] *= rstd;
+              dw[i][j] += v[i][j] * x[i][j];
+              db[i][j] += v[i][j];
+              v[i][j] *= sw[e + j];
+              gn += v[i][j] * x[i][j];
+              gs += v[i][j];
+            }
+          }
+        }
+        gn = group_sum<G>(gn) * p.inv_norm_dim;
+        gs = sd.norm == kNormLayer ? group_sum<G>(gs) * p.inv_norm_dim : 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = rstd * (v[i][j] - gn * x[i][j] - gs);
+          }
+      }
+      if (live) {
+        T* dx = static_cast<T*>(sd.y) + (static_cast<long long>(token) * sd.H + head) * p.D;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (lane + G * i < units) *reinterpret_cast<uint4*>(dx + (lane + G * i) * 8) = pack8<T>(v[i]);
+      }
+    }
+  }
+  if constexpr (kNorm) {
+    if (!sd.partials) return;
+    // the groups of the block add their sums one after the other: the same order in every run
+    for (int turn = 0; turn < kGroups; ++turn) {
+      __syncthreads();
+      if (group == turn) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int e = (lane + G * i) * 8;
+          if (e < p.norm_dim) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { sdw[e + j] += dw[i][j]; sdb[e + j] += db[i][j]; }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    float* line = sd.partials + static_cast<long long>(blockIdx.x) * 2 * p.norm_dim;
+    for (int i = tid; i < p.norm_dim; i += kThreads) { line[i] = sdw[i]; line[p.norm_dim + i] = sdb[i]; }
+  }
+}
+
+// dweight and dbias from the blocks' lines: a block takes 32 columns of the 2 * norm_dim, its warps every eighth line.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_rope_param_grad_kernel(const float* partials, int lines, int norm_dim, void* d_weight, void* d_bias, int fp32) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < 2 * norm_dim)
+    for (int l = warp; l < lines; l += 8) s += partials[static_cast<long long>(l) * 2 * norm_dim + c];
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < 2 * norm_dim) {
+    s = 0.f;
+    for (int w = 0; w < 8; ++w) s += sums[w][lane];
+    void* out = c < norm_dim ? d_weight : d_bias;
+    const int i = c < norm_dim ? c : c - norm_dim;
+    if (out) {
+      if (fp32) static_cast<float*>(out)[i] = s;
+      else static_cast<T*>(out)[i] = static_cast<T>(s);
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------
+// any size, offset and stride: a warp per row, element by element.  kBack: backward (dweight / dbias sums through the lines of
+// the workspace, one per block, added by one warp of the block after the other).
+// -------------------------------------------------------------------------------------------------
+namespace nr {
+template <typename T>
+__device__ __forceinline__ void any_stats(const NormRopeParams& p, const RopeSide& sd, const T* x, int lane, float* mean, float* rstd) {
+  const int n = p.norm_dim;
+  *mean = 0.f;
+  *rstd = 1.f;
+  if (!sd.norm) return;
+  if (sd.norm == kNormLayer) {
+    float s = 0.f;
+    for (int e = lane; e < n; e += 32) s += static_cast<float>(x[e]);
+    *mean = group_sum<32>(s) * p.inv_norm_dim;
+  }
+  float q = 0.f;
+  for (int e = lane; e < n; e += 32) { const float d = static_cast<float>(x[e]) - *mean; q += d * d; }
+  *rstd = rsqrtf(group_sum<32>(q) * p.inv_norm_dim + p.eps);
+}
+
+// Element e of the rotated row (dir = -1: rotated back) whose elements `at` gives.
+template <typename At>
+__device__ __forceinline__ float any_rotated(const NormRopeParams& p, long long position, int e, float dir, At at) {
+  const int d = e - p.rope_start, half = p.R >> 1;
+  if (d < 0 || d >= p.R) return at(e);
+  const bool second = p.interleaved ? (d & 1) != 0 : d >= half;
+  const int pair = p.interleaved ? d >> 1 : (second ? d - half : d);
+  const int partner = p.interleaved ? p.rope_start + (d ^ 1) : (second ? e - half : e + half);
+  const float2 t = turn_of(position, p.inv_freq[pair], p.rope_scale);
+  return at(e) * t.x + at(partner) * (second ? dir * t.y : -dir * t.y);
+}
+
+template <typename T, bool kBack>
+__device__ __forceinline__ void any_row(const NormRopeParams& p, const RopeSide& sd, long long r, int token, int head, int lane) {
+  const T* x = row_of<T>(sd.x, p.S, token, head);
+  const int n = p.norm_dim;
+  const long long position = position_of(p, token);
+  float mean = 0.f, rstd = 1.f;
+  if (sd.norm) any_stats(p, sd, x, lane, &mean, &rstd);
+  auto weight = [&](int e) { return sd.weight ? param_at<T>(sd.weight, sd.param_fp32, e) : 1.f; };
+  if constexpr (!kBack) {
+    const long long orow = out_row(sd, token, head);
+    if (orow < 0) return;
+    auto normed = [&](int e) {
+      const float v = static_cast<float>(x[e]);
+      if (!sd.norm || e >= n) return v;
+      return (v - mean) * rstd * weight(e) + (sd.bias ? param_at<T>(sd.bias, sd.param_fp32, e) : 0.f);
+    };
+    for (int e = lane; e < p.D; e += 32) {
+      T* y = e < sd.split ? static_cast<T*>(sd.y) + orow * sd.split + e : static_cast<T*>(sd.y_tail) + orow * (p.D - sd.split) + (e - sd.split);
+      *y = static_cast<T>(any_rotated(p, position, e, 1.f, normed));
+    }
+  } else {
+    const T* dy = row_of<T>(sd.dy, p.S, token, head);
+    auto grad = [&](int e) { return static_cast<float>(dy[e]); };
+    float gn = 0.f, gs = 0.f;
+    if (sd.norm) {
+      for (int e = lane; e < n; e += 32) {
+        const float u = any_rotated(p, position, e, -1.f, grad) * weight(e);
+        gn += u * (static_cast<float>(x[e]) - mean) * rstd;
+        gs += u;
+      }
+      gn = group_sum<32>(gn) * p.inv_norm_dim;
+      gs = sd.norm == kNormLayer ? group_sum<32>(gs) * p.inv_norm_dim : 0.f;
+    }
+    T* dx = static_cast<T*>(sd.y) + r * p.D;
+    for (int e = lane; e < p.D; e += 32) {
+      float u = any_rotated(p, position, e, -1.f, grad);
+      if (sd.norm && e < n) u = rstd * (u * weight(e) - gn * (static_cast<float>(x[e]) - mean) * rstd - gs);
+      dx[e] = static_cast<T>(u);
+    }
+  }
+}
+}  // namespace nr
+
+template <typename T, bool kBack>
+__global__ void __launch_bounds__(nr::kThreads) norm_rope_any_kernel(const __grid_constant__ NormRopeParams p) {
+  using namespace nr;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kThreads / 32;
+  const long long rows0 = static_cast<long long>(p.tokens) * p.side[0].H, rows1 = kBack ? 0 : static_cast<long long>(p.tokens) * p.side[1].H;
+  float* line = kBack && p.side[0].partials ? p.side[0].partials + static_cast<long long>(blockIdx.x) * 2 * p.norm_dim : nullptr;
+  if (line) {
+    for (int i = threadIdx.x; i < 2 * p.norm_dim; i += kThreads) line[i] = 0.f;
+    __syncthreads();
+  }
+  const long long total = rows0 + rows1, step = static_cast<long long>(gridDim.x) * warps;
+  for (long long base = static_cast<long long>(blockIdx.x) * warps; base < total; base += step) {
+    const long long g = base + warp;
+    if (g < total) {
+      const RopeSide& sd = p.side[g >= rows0 ? 1 : 0];
+      const long long r = g >= rows0 ? g - rows0 : g;
+      const int token = static_cast<int>(r / sd.H), head = static_cast<int>(r - static_cast<long long>(token) * sd.H);
+      any_row<T, kBack>(p, sd, r, token, head, lane);
+    }
+    if (line)   // the block's warps add their rows' sums one after the other
+      for (int turn = 0; turn < warps; ++turn) {
+        __syncthreads();
+        if (warp == turn && g < total) {
+          const RopeSide& sd = p.side[0];
+          const int token = static_cast<int>(g / sd.H), head = static_cast<int>(g - static_cast<long long>(token) * sd.H);
+          const T* x = row_of<T>(sd.x, p.S, token, head);
+          const T* dy = row_of<T>(sd.dy, p.S, token, head);
+          float mean, rstd;
+          any_stats(p, sd, x, lane, &mean, &rstd);
+          const long long position = position_of(p, token);
+          for (int e = lane; e < p.norm_dim; e += 32) {
+            const float u = any_rotated(p, position, e, -1.f, [&](int i) { return static_cast<float>(dy[i]); });
+            line[e] += u * (static_cast<float>(x[e]) - mean) * rstd;
+            line[p.norm_dim + e] += u;
+          }
+        }
+      }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------
+// host side
+// -------------------------------------------------------------------------------------------------
+namespace {
+bool aligned_view(const RowView& v) {
+  return !v.base || ((reinterpret_cast<uintptr_t>(v.base) & 15u) == 0 && v.stride_b % 8 == 0 && v.stride_s % 8 == 0 && v.stride_h % 8 == 0);
+}
+// Do all rows come in 16-byte units?
+bool in_units(const NormRopeParams& p) {
+  if (p.D % 8 || p.D > nr::kMaxNormDim || p.rope_start % 8 || p.R % (p.interleaved ? 8 : 16) || p.norm_dim % 8 || p.R / 2 > nr::kMaxPairs) return false;
+  for (const RopeSide& sd : p.side) {
+    if (!sd.H) continue;
+    if (!aligned_view(sd.x) || !aligned_view(sd.dy) || sd.split % 8) return false;
+    if ((reinterpret_cast<uintptr_t>(sd.y) | reinterpret_cast<uintptr_t>(sd.y_tail)) & 15u) return false;
+  }
+  return true;
+}
+// Tokens x heads of a block: at most `rows` rows; one token's heads first (they share its angles).
+void tile(NormRopeParams* p, int which, int rows) {
+  RopeSide& sd = p->side[which];
+  if (!sd.H) { sd.blocks = 0; sd.tile_heads = sd.tile_tokens = 1; return; }
+  sd.tile_heads = sd.H < rows ? sd.H : rows;
+  int tokens = rows / sd.tile_heads;
+  const int most = nr::kMaxPairs / (p->R / 2);
+  if (tokens > most) tokens = most;
+  if (tokens > p->tokens) tokens = p->tokens;
+  sd.tile_tokens = tokens < 1 ? 1 : tokens;
+  sd.blocks = ((p->tokens + sd.tile_tokens - 1) / sd.tile_tokens) * ((sd.H + sd.tile_heads - 1) / sd.tile_heads);
+}
+// Rows per block: 64 amortise a block's angles and weights; calls that would not fill the SMs twice take shorter blocks.
+void tiles(NormRopeParams* p, int sms) {
+  for (int rows = 64; rows >= 8; rows >>= 1) {
+    tile(p, 0, rows);
+    tile(p, 1, rows);
+    if (p->side[0].blocks + p->side[1].blocks >= 2 * sms) return;
+  }
+}
+int tile_smem(const NormRopeParams& p) {
+  int tokens = 1;
+  for (const RopeSide& sd : p.side)
+    if (sd.H && sd.tile_tokens > tokens) tokens = sd.tile_tokens;
+  return tokens * (p.R / 2) * static_cast<int>(sizeof(float2));
+}
+
+template <typename T, int G, int NV>
+int forward(const NormRopeParams& p, cudaStream_t stream) {
+  norm_rope_kernel<T, G, NV><<<p.side[0].blocks + p.side[1].blocks, nr::kThreads, tile_smem(p), stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T, int G, int NV>
+int backward(const NormRopeParams& p, int grid, cudaStream_t stream) {
+  if (p.side[0].norm) norm_rope_bwd_kernel<T, G, NV, true><<<grid, nr::kThreads, tile_smem(p), stream>>>(p);
+  else norm_rope_bwd_kernel<T, G, NV, false><<<grid, nr::kThreads, tile_smem(p), stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T>
+int forward_units(const NormRopeParams& p, cudaStream_t stream) {
+  if (p.D <= 64) return forward<T, 8, 1>(p, stream);
+  if (p.D <= 128) return forward<T, 16, 1>(p, stream);
+  if (p.D <= 256) return forward<T, 32, 1>(p, stream);
+  if (p.D <= 512) return forward<T, 32, 2>(p, stream);
+  if (p.D <= 768) return forward<T, 32, 3>(p, stream);
+  return forward<T, 32, 4>(p, stream);
+}
+template <typename T>
+int backward_units(const NormRopeParams& p, int grid, cudaStream_t stream) {
+  if (p.D <= 64) return backward<T, 8, 1>(p, grid, stream);
+  if (p.D <= 128) return backward<T, 16, 1>(p, grid, stream);
+  if (p.D <= 256) return backward<T, 32, 1>(p, grid, stream);
+  if (p.D <= 512) return backward<T, 32, 2>(p, grid, stream);
+  if (p.D <= 768) return backward<T, 32, 3>(p, grid, stream);
+  return backward<T, 32, 4>(p, grid, stream);
+}
+// Blocks of a backward with a norm: every block leaves one line of sums.
+int norm_lines(int sms) { return 4 * sms; }
+}  // namespace
+
+int launch_norm_rope(NormRopeParams p, bool bf16, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  cudaError_t e = current_device_sms(&dev, &sms);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (!in_units(p)) {
+    const long long rows = static_cast<long long>(p.tokens) * (p.side[0].H + p.side[1].H), want = (rows + 7) / 8;
+    const int grid = static_cast<int>(want < 8LL * sms ? want : 8LL * sms);
+    if (bf16) norm_rope_any_kernel<__nv_bfloat16, false><<<grid, nr::kThreads, 0, stream>>>(p);
+    else norm_rope_any_kernel<__half, false><<<grid, nr::kThreads, 0, stream>>>(p);
+    return static_cast<int>(cudaGetLastError());
+  }
+  tiles(&p, sms);
+  return bf16 ? forward_units<__nv_bfloat16>(p, stream) : forward_units<__half>(p, stream);
+}
+
+size_t norm_rope_bwd_workspace_bytes(int norm_dim) {
+  int dev = 0, sms = 0;
+  if (current_device_sms(&dev, &sms) != cudaSuccess) return 0;
+  return static_cast<size_t>(norm_lines(sms)) * 2 * norm_dim * sizeof(float);
+}
+
+// p.side[0]: x (norm only), dy, y = dx, partials = workspace when dweight or dbias is asked for.
+int launch_norm_rope_bwd(NormRopeParams p, void* d_weight, void* d_bias, bool bf16, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  cudaError_t e = current_device_sms(&dev, &sms);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  int grid, err;
+  if (!in_units(p)) {
+    const long long want = (static_cast<long long>(p.tokens) * p.side[0].H + 7) / 8;
+    grid = static_cast<int>(want < norm_lines(sms) ? want : norm_lines(sms));
+    if (bf16) norm_rope_any_kernel<__nv_bfloat16, true><<<grid, nr::kThreads, 0, stream>>>(p);
+    else norm_rope_any_kernel<__half, true><<<grid, nr::kThreads, 0, stream>>>(p);
+    err = static_cast<int>(cudaGetLastError());
+  } else {
+    tiles(&p, sms);
+    grid = p.side[0].norm && p.side[0].blocks > norm_lines(sms) ? norm_lines(sms) : p.side[0].blocks;
+    err = bf16 ? backward_units<__nv_bfloat16>(p, grid, stream) : backward_units<__half>(p, grid, stream);
+  }
+  if (err || !p.side[0].partials) return err;
+  const int cols = (2 * p.norm_dim + 31) / 32;
+  if (bf16) norm_rope_param_grad_kernel<__nv_bfloat16><<<cols, 256, 0, stream>>>(p.side[0].partials, grid, p.norm_dim, d_weight, d_bias, p.side[0].param_fp32);
+  else norm_rope_param_grad_kernel<__half><<<cols, 256, 0, stream>>>(p.side[0].partials, grid, p.norm_dim, d_weight, d_bias, p.side[0].param_fp32);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace dsa
