@@ -323,6 +323,22 @@ int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stri
                       int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps,
                       void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
 
+/* Distillation of rows of logits from a teacher's top entries: student [rows, V] (rows row_stride elements apart), teacher [rows, K],
+ * indices [rows, K] int32 columns of the entries (NULL: K = V, entry j is column j).  An entry takes part when its column lies in
+ * [0, V) and the student's logit there is not -inf; p = the teacher's entries (weights, or exp(logit / temperature) when
+ * teacher_logits) over their sum, s = softmax(student / temperature) over the participating entries, or over the whole row when
+ * over_row: loss [rows] fp32 = sum p (log p - log s), 0 for rows without teacher weight.  stats [rows, 4] fp32 (16-byte aligned) is
+ * what the backward needs.  dtypes: 0 bfloat16, 1 float16, 2 float32.  No reference counterpart. */
+int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,
+                          const int32_t* indices, float* loss, float* stats, int64_t rows, int32_t V, int32_t K, int32_t over_row,
+                          int32_t teacher_logits, float temperature, void* stream);
+
+/* Its gradient: grad [rows] fp32, d_student [rows, V] contiguous (the student's type), every column written.  A column that a row
+ * lists more than once gets the sum of its entries (of three or more in no fixed order). */
+int dsa_topk_distillation_bwd(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,
+                              const int32_t* indices, const float* stats, const float* grad, void* d_student, int64_t rows, int32_t V,
+                              int32_t K, int32_t over_row, int32_t teacher_logits, float temperature, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

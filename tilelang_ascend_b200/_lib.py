@@ -87,6 +87,10 @@ SIGNATURES = {
     "dsa_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int32]),
     "dsa_norm_rope_bwd": (c_int32, [ctypes.POINTER(RopeRows), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p] + [c_int32] * 7
                           + [c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_int32, c_void_p]),
+    "dsa_topk_distillation": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64] + [c_int32] * 4
+                              + [c_float, c_void_p]),
+    "dsa_topk_distillation_bwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64]
+                                  + [c_int32] * 4 + [c_float, c_void_p]),
 }
 
 _lib = None

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "../../include/dsa_b200.h"
+#include "distill.h"
 #include "launch_util.h"
 #include "norm_rope.h"
 #include "params.h"
@@ -136,6 +137,23 @@ int fill_rope_side(dsa::RopeSide* sd, const dsa_rope_rows* r, int32_t D, int32_t
   sd->x = dsa::RowView{r->x, r->stride_b, r->stride_s, r->stride_h};
   sd->H = r->heads; sd->norm = r->norm; sd->weight = r->weight; sd->bias = r->bias; sd->param_fp32 = r->params_fp32;
   sd->y = r->y; sd->y_tail = r->y_tail; sd->split = r->split; sd->slots = r->slots; sd->slots64 = r->slots_int64; sd->y_slots = r->y_slots;
+  return 0;
+}
+
+int fill_distill(dsa::DistillParams* p, const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,
+                 const int32_t* indices, const float* stats, int64_t rows, int32_t V, int32_t K, int32_t over_row, int32_t teacher_logits, float temperature) {
+  if (!student || !teacher || !stats) return fail("null tensor pointer");
+  if (student_dtype < 0 || student_dtype > 2 || teacher_dtype < 0 || teacher_dtype > 2) return fail("dtypes must be 0 (bfloat16), 1 (float16) or 2 (float32)");
+  if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || K <= 0 || V > 0x7fffffff - 65536) return fail("rows, V and K must be positive (rows and V below 2^31)");
+  if (!indices && K != V) return fail("without indices K must equal V");
+  if (!(temperature > 0.f) || !std::isfinite(temperature)) return fail("temperature must be positive and finite");
+  if (reinterpret_cast<uintptr_t>(stats) & 15u) return fail("stats must be 16-byte aligned");
+  *p = dsa::DistillParams{};
+  p->student = student; p->teacher = teacher; p->indices = indices; p->stats = const_cast<float*>(stats);
+  p->rows = rows; p->row_stride = row_stride; p->V = V; p->K = K;
+  p->student_type = student_dtype; p->teacher_type = teacher_dtype; p->teacher_logits = teacher_logits ? 1 : 0; p->over_row = over_row ? 1 : 0;
+  p->inv_T = 1.f / temperature;
+  p->exp_scale = static_cast<float>(1.4426950408889634 / temperature);
   return 0;
 }
 
@@ -598,6 +616,29 @@ int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stri
   }
   int err = dsa::launch_norm_rope_bwd(p, d_weight, d_bias, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("norm_rope_bwd launch", err) : 0;
+}
+
+int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype, const int32_t* indices,
+                          float* loss, float* stats, int64_t rows, int32_t V, int32_t K, int32_t over_row, int32_t teacher_logits, float temperature,
+                          void* stream) {
+  dsa::DistillParams p;
+  if (!loss) return fail("null output pointer");
+  if (fill_distill(&p, student, student_dtype, row_stride, teacher, teacher_dtype, indices, stats, rows, V, K, over_row, teacher_logits, temperature)) return 1;
+  p.loss = loss;
+  int err = dsa::launch_distill_fwd(p, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("topk_distillation launch", err) : 0;
+}
+
+int dsa_topk_distillation_bwd(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,
+                              const int32_t* indices, const float* stats, const float* grad, void* d_student, int64_t rows, int32_t V, int32_t K,
+                              int32_t over_row, int32_t teacher_logits, float temperature, void* stream) {
+  dsa::DistillParams p;
+  if (!grad || !d_student) return fail("null tensor pointer");
+  if (fill_distill(&p, student, student_dtype, row_stride, teacher, teacher_dtype, indices, stats, rows, V, K, over_row, teacher_logits, temperature)) return 1;
+  p.grad = grad;
+  p.d_student = d_student;
+  int err = dsa::launch_distill_bwd(p, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("topk_distillation_bwd launch", err) : 0;
 }
 
 }  // extern "C"

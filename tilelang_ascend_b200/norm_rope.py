@@ -13,6 +13,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .adapter import current_stream, dtype_code, ptr
@@ -141,6 +142,7 @@ class QkNormRopeFunction(torch.autograd.Function):
         return tuple(outs)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *d_outs):
         q, k, q_weight, q_bias, k_weight, k_bias, positions, inv_freq = ctx.saved_tensors
         rope_start, interleaved, rope_scale, q_norm, k_norm, norm_dim, eps = ctx.rest
