@@ -339,6 +339,21 @@ int dsa_topk_distillation_bwd(const void* student, int32_t student_dtype, int64_
                               const int32_t* indices, const float* stats, const float* grad, void* d_student, int64_t rows, int32_t V,
                               int32_t K, int32_t over_row, int32_t teacher_logits, float temperature, void* stream);
 
+/* Attention weights of the listed keys, averaged over the heads: weights [B, S, 1, topk] fp32 = 1 / H sum_h exp(sm_scale q[h] . kv[idx] -
+ * lse[h]), 0 for entries that take no part (the rules of dsa_sparse_mla_fwd); lse [B, S, H] fp32 is the forward's (a head with
+ * -inf has no weight).  q [B, S, H, D], kv [B, S_kv, 1, D] 16-byte aligned, D a multiple of 8, at most 640; topk at most 8192.  No
+ * reference counterpart (the indexer's teacher). */
+int dsa_sparse_mla_key_weights(const void* q, const void* kv, const int32_t* indices, const float* lse, float* weights, int32_t B, int32_t S,
+                               int32_t S_kv, int32_t H, int32_t D, int32_t topk, float sm_scale, int32_t q_start, int32_t causal,
+                               int32_t dtype, void* stream);
+
+/* Backward of the indexer's scores at listed keys: q [B, S1, N1, 128], k [B, S2, 1, 128], w [B, S1, N1] fp32, indices [B, S1, 1, K]
+ * (entries outside [0, S2) take no part), grad [B, S1, 1, K] fp32 of the scores there.  d_q (inputs' type) and d_w (fp32) are
+ * written, d_k [B, S2, 1, 128] fp32 is added to (the order of its additions is not fixed).  N1 at most 64, K at most 8192; q and k
+ * 16-byte aligned.  relu'(0) = 0.  No reference counterpart. */
+int dsa_lightning_indexer_bwd(const void* q, const void* k, const float* w, const int32_t* indices, const float* grad, void* d_q, float* d_k,
+                              float* d_w, int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

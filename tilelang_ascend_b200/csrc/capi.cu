@@ -8,6 +8,7 @@
 
 #include "../../include/dsa_b200.h"
 #include "distill.h"
+#include "indexer_bwd.h"
 #include "launch_util.h"
 #include "norm_rope.h"
 #include "params.h"
@@ -42,6 +43,8 @@ int launch_v4_build_joined_indices(const int32_t* cu_q, const int32_t* seqused_k
 int launch_bounded_wait_selftest(int* status, long long budget_cycles, int* gave_up, cudaStream_t stream);
 bool sparse_mla_bwd_tc_supported(const FwdParams& p);
 size_t sparse_mla_bwd_tc_bytes_per_query(int H, int topk);
+bool sparse_mla_key_weights_supported(const FwdParams& p);
+int launch_sparse_mla_key_weights(const FwdParams& p, float* weights, bool bf16, cudaStream_t stream);
 int launch_sparse_mla_bwd_tc(const BwdParams& bp, bool bf16, void* workspace, size_t workspace_bytes, int queries_per_pass, cudaStream_t stream);
 }  // namespace dsa
 
@@ -639,6 +642,33 @@ int dsa_topk_distillation_bwd(const void* student, int32_t student_dtype, int64_
   p.d_student = d_student;
   int err = dsa::launch_distill_bwd(p, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("topk_distillation_bwd launch", err) : 0;
+}
+
+int dsa_sparse_mla_key_weights(const void* q, const void* kv, const int32_t* indices, const float* lse, float* weights, int32_t B, int32_t S, int32_t S_kv,
+                               int32_t H, int32_t D, int32_t topk, float sm_scale, int32_t q_start, int32_t causal, int32_t dtype, void* stream) {
+  if (!lse) return fail("null tensor pointer");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv)) & 15u) return fail("q and kv must be 16-byte aligned");
+  dsa::FwdParams p;
+  if (fill_fwd_params(&p, q, kv, indices, weights, const_cast<float*>(lse), B, S, S_kv, H, D, 1, topk, sm_scale, q_start, causal, dtype, nullptr, nullptr,
+                      nullptr, nullptr, 0, 0))
+    return 1;
+  if (!dsa::sparse_mla_key_weights_supported(p)) return fail("lists of at most 8192 keys");
+  int err = dsa::launch_sparse_mla_key_weights(p, weights, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("sparse_mla_key_weights launch", err) : 0;
+}
+
+int dsa_lightning_indexer_bwd(const void* q, const void* k, const float* w, const int32_t* indices, const float* grad, void* d_q, float* d_k, float* d_w,
+                              int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype, void* stream) {
+  if (!q || !k || !w || !indices || !grad || !d_q || !d_k || !d_w) return fail("null tensor pointer");
+  if (!dtype_ok(dtype)) return fail("dtype must be 0 (bfloat16) or 1 (float16)");
+  if (B <= 0 || S1 <= 0 || S2 <= 0 || N1 <= 0 || K <= 0) return fail("B, S1, S2, N1 and K must be positive");
+  if (static_cast<int64_t>(B) * S1 > 0x3fffffffLL) return fail("B * S1 too large");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k)) & 15u) return fail("q and k must be 16-byte aligned");
+  dsa::IndexerBwdParams p{q, k, w, indices, grad, d_q, d_k, d_w, B, S1, S2, N1, D, K, nullptr};
+  if (!dsa::indexer_bwd_supported(p)) return fail("the indexer's backward needs D = 128, at most 64 heads and lists of at most 8192 keys");
+  if (get_status_word(&p.status)) return 1;
+  int err = dsa::launch_indexer_bwd(p, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  return err ? fail_cuda("lightning_indexer_bwd launch", err) : 0;
 }
 
 }  // extern "C"

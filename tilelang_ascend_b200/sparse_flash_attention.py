@@ -348,3 +348,31 @@ def sparse_mla(q, kv, indices, sm_scale=None, q_start_index_s=None, dv=512):
     scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
     q_start = kv.shape[1] - q.shape[1] if q_start_index_s is None else int(q_start_index_s)
     return SparseMLAFunction.apply(q, kv, indices, scale, q_start, dv)
+
+
+def sparse_mla_key_weights(q, kv, indices, lse, *, sm_scale: Optional[float] = None, q_start_index_s: Optional[int] = None):
+    """What the softmax of :func:`sparse_mla` gives the keys of every query's list, averaged over the heads: fp32 [B,S,1,topk],
+    ``mean_h exp(sm_scale * q[h] . kv[idx] - lse[h])`` -- the teacher the lightning indexer is trained with
+    (:func:`lightning_indexer_distillation`).  No reference counterpart.
+
+    q [B,S,H,D], kv [B,S_kv,1,D] (D a multiple of 8, at most 640), indices [B,S,1,topk] int32 (at most 8192 entries; -1, beyond S_kv or
+    beyond the query's position: weight 0) and lse [B,S,H] fp32 as :func:`sparse_mla` takes and returns them, with the same
+    ``sm_scale`` and ``q_start_index_s``.  A list that names a key twice gives each entry the key's weight.  No gradient flows through
+    a teacher: the result never requires one."""
+    code = dtype_code(q.dtype)
+    if q.dim() != 4 or kv.dim() != 4 or indices.dim() != 4:
+        raise ValueError("q, kv and indices must be 4-dimensional ([B,S,H,D], [B,S_kv,1,D], [B,S,1,topk])")
+    B, S, H, D = q.shape
+    S_kv, topk = kv.shape[1], indices.shape[3]
+    if kv.shape != (B, S_kv, 1, D) or indices.shape[:3] != (B, S, 1) or lse.shape != (B, S, H):
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, kv {tuple(kv.shape)}, indices {tuple(indices.shape)}, lse {tuple(lse.shape)}")
+    if D % 8 or not 0 < D <= 640 or not 0 < topk <= 8192 or H < 1 or S_kv < 1:
+        raise ValueError(f"D must be a multiple of 8, at most 640, topk in [1, 8192], H and S_kv positive (got D {D}, topk {topk}, H {H}, S_kv {S_kv})")
+    dev = check_inputs([q, kv, indices, lse], [None, q.dtype, torch.int32, torch.float32], ["q", "kv", "indices", "lse"])
+    weights = torch.empty((B, S, 1, topk), dtype=torch.float32, device=dev)
+    if B * S:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().dsa_sparse_mla_key_weights(
+                ptr(q), ptr(kv), ptr(indices), ptr(lse), ptr(weights), B, S, S_kv, H, D, topk, float(D ** -0.5 if sm_scale is None else sm_scale),
+                S_kv - S if q_start_index_s is None else int(q_start_index_s), 1, code, current_stream(dev)))
+    return weights
