@@ -314,14 +314,22 @@ int dsa_norm_rope(const dsa_rope_rows* q, const dsa_rope_rows* k, const void* po
                   int32_t B, int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved,
                   float rope_scale, float eps, int32_t dtype, void* stream);
 
-/* Gradients of one side: rows->x (read with a norm only), rows->y = dx [B, S, heads, D] contiguous; dy with unit inner stride.
- * d_weight / d_bias [norm_dim] (the parameters' type) or NULL; when one is given, workspace holds at least
- * dsa_norm_rope_bwd_workspace_bytes(norm_dim) bytes.  Sums are taken in a fixed order. */
+/* Gradients of queries or keys: rows.x is read with a norm only, rows.y = dx [B, S, heads, D] contiguous, dy with unit inner stride;
+ * d_weight / d_bias [norm_dim] (the parameters' type) or NULL. */
+typedef struct dsa_rope_grads {
+  dsa_rope_rows rows;
+  const void* dy;
+  int64_t dy_stride_b, dy_stride_s, dy_stride_h;
+  void* d_weight;
+  void* d_bias;
+} dsa_rope_grads;
+
+/* Backward of dsa_norm_rope.  workspace: dsa_norm_rope_bwd_workspace_bytes(norm_dim) for each of q and k that asks for d_weight or
+ * d_bias.  Those sums are taken in a fixed order. */
 size_t dsa_norm_rope_bwd_workspace_bytes(int32_t norm_dim);
-int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stride_b, int64_t dy_stride_s, int64_t dy_stride_h,
-                      const void* positions, int32_t positions_int64, const float* inv_freq, int32_t B, int32_t S, int32_t D,
-                      int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps,
-                      void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
+int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const void* positions, int32_t positions_int64, const float* inv_freq,
+                      int32_t B, int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved,
+                      float rope_scale, float eps, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
 
 /* Distillation of rows of logits from a teacher's top entries: student [rows, V] (rows row_stride elements apart), teacher [rows, K],
  * indices [rows, K] int32 columns of the entries (NULL: K = V, entry j is column j).  An entry takes part when its column lies in

@@ -272,11 +272,11 @@ def test_training_step_of_an_indexer():
     soft = torch.softmax(values.double(), -1)
     d_values = ((soft - p) / (B * S)).masked_fill(indices < 0, 0.0).cpu()
     want, _ = indexer_gradients(qi.detach().cpu(), ki.detach().cpu(), head_w.detach().cpu(), indices.cpu(), d_values)
-    dx, _, _ = dsa.qk_norm_rope_bwd_raw(want["q"].to(torch.bfloat16).cuda(), None, positions, inv_freq, interleaved=False)
+    dx = dsa.qk_norm_rope_bwd_raw(want["q"].to(torch.bfloat16).cuda(), None, None, None, positions, inv_freq, interleaved=False)[0]
     # dz, the result, and the rows behind the rotation are rounded once each on either side
     assert float((raw["qi"].grad.double() - dx.double()).norm()) <= 4 * 2.0 ** -8 * float(dx.double().norm())
-    dk, dlw, dlb = dsa.qk_norm_rope_bwd_raw(want["k"].to(torch.bfloat16).cuda(), raw["ki"].detach(), positions, inv_freq, interleaved=False, norm="layer",
-                                            weight=ln_w.detach(), bias=ln_b.detach())
+    _, dk, _, _, dlw, dlb = dsa.qk_norm_rope_bwd_raw(None, want["k"].to(torch.bfloat16).cuda(), None, raw["ki"].detach(), positions, inv_freq,
+                                                     interleaved=False, k_norm="layer", k_weight=ln_w.detach(), k_bias=ln_b.detach())
     for got, ref in ((raw["ki"].grad, dk), (ln_w.grad, dlw), (ln_b.grad, dlb)):
         assert float((got.double() - ref.double()).norm()) <= 4 * 2.0 ** -8 * float(ref.double().norm())
     assert float((head_w.grad.cpu().double() - want["w"]).norm()) <= 2.0 ** -12 * float(want["w"].norm())

@@ -253,7 +253,8 @@ def test_repeatable_captured_and_on_another_stream():
 
     def step():
         oq, ok = dsa.qk_norm_rope(q, k, positions, inv_freq, q_norm="rms", k_norm="rms", q_weight=weight, interleaved=False)
-        return (oq, ok) + dsa.qk_norm_rope_bwd_raw(d, q, positions, inv_freq, norm="rms", weight=weight, interleaved=False)[:2]
+        grads = dsa.qk_norm_rope_bwd_raw(d, k * 0.5, q, None, positions, inv_freq, q_norm="rms", q_weight=weight, interleaved=False)
+        return (oq, ok) + grads[:3]
 
     first = step()
     assert all(torch.equal(a, b) for a, b in zip(first, step()))
@@ -305,7 +306,9 @@ def test_refusals():
         lambda: dsa.qk_norm_rope_cached(q, k, pos, f, cache.half(), slots),
         lambda: dsa.qk_norm_rope_cached(q, k, pos, f, cache[:, ::2], slots),
         lambda: dsa.qk_norm_rope_cached(q.requires_grad_(), k, pos, f, cache, slots),
-        lambda: dsa.qk_norm_rope_bwd_raw(k, q.detach(), pos, f, norm="rms"),
+        lambda: dsa.qk_norm_rope_bwd_raw(k, None, q.detach(), None, pos, f, q_norm="rms"),
+        lambda: dsa.qk_norm_rope_bwd_raw(k, None, None, None, pos, f, q_norm="rms"),
+        lambda: dsa.qk_norm_rope_bwd_raw(None, None, q.detach(), k, pos, f),
     ]
     for call in bad:
         with pytest.raises(ValueError) as e:
@@ -320,4 +323,4 @@ def test_c_entry_refuses_before_any_cuda_call():
     lib = _lib.load()
     scalars = (None, 0, None, 1, 1, 64, 32, 0, 0, 1, 1.0, 1e-6)
     assert lib.dsa_norm_rope(None, None, *scalars, 0, None) != 0 and b"given" in lib.dsa_get_last_error()
-    assert lib.dsa_norm_rope_bwd(None, None, 0, 0, 0, *scalars, None, None, None, 0, 0, None) != 0
+    assert lib.dsa_norm_rope_bwd(None, None, *scalars, None, 0, 0, None) != 0

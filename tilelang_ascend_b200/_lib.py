@@ -24,6 +24,12 @@ class RopeRows(ctypes.Structure):
                 ("slots", c_void_p), ("y_slots", c_int64), ("slots_int64", c_int32), ("reserved", c_int32)]
 
 
+class RopeGrads(ctypes.Structure):
+    """``dsa_rope_grads`` of the C header."""
+    _fields_ = [("rows", RopeRows), ("dy", c_void_p), ("dy_stride_b", c_int64), ("dy_stride_s", c_int64), ("dy_stride_h", c_int64),
+                ("d_weight", c_void_p), ("d_bias", c_void_p)]
+
+
 # name -> (restype, argtypes); must list every symbol include/dsa_b200.h declares
 SIGNATURES = {
     "dsa_init": (c_int32, []),
@@ -85,8 +91,8 @@ SIGNATURES = {
     "dsa_norm_rope": (c_int32, [ctypes.POINTER(RopeRows), ctypes.POINTER(RopeRows), c_void_p, c_int32, c_void_p] + [c_int32] * 7
                       + [c_float, c_float, c_int32, c_void_p]),
     "dsa_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int32]),
-    "dsa_norm_rope_bwd": (c_int32, [ctypes.POINTER(RopeRows), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p] + [c_int32] * 7
-                          + [c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_int32, c_void_p]),
+    "dsa_norm_rope_bwd": (c_int32, [ctypes.POINTER(RopeGrads), ctypes.POINTER(RopeGrads), c_void_p, c_int32, c_void_p] + [c_int32] * 7
+                          + [c_float, c_float, c_void_p, c_size_t, c_int32, c_void_p]),
     "dsa_topk_distillation": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64] + [c_int32] * 4
                               + [c_float, c_void_p]),
     "dsa_topk_distillation_bwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64]

@@ -7,6 +7,7 @@ launches on the current stream.  The helpers here reproduce those rules for the 
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Optional, Sequence
 
 import torch
@@ -59,3 +60,16 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def current_stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+_HERE = nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context in which ``dev`` is the current device; does nothing when it is already (a device switch costs a small call's launch)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def raw_stream(dev: torch.device) -> int:
+    """:func:`current_stream` without the stream object in between."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)

@@ -602,20 +602,32 @@ int dsa_norm_rope(const dsa_rope_rows* q, const dsa_rope_rows* k, const void* po
 
 size_t dsa_norm_rope_bwd_workspace_bytes(int32_t norm_dim) { return norm_dim > 0 ? dsa::norm_rope_bwd_workspace_bytes(norm_dim) : 0; }
 
-int dsa_norm_rope_bwd(const dsa_rope_rows* rows, const void* dy, int64_t dy_stride_b, int64_t dy_stride_s, int64_t dy_stride_h, const void* positions,
-                      int32_t positions_int64, const float* inv_freq, int32_t B, int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start,
-                      int32_t norm_dim, int32_t interleaved, float rope_scale, float eps, void* d_weight, void* d_bias, void* workspace,
-                      size_t workspace_bytes, int32_t dtype, void* stream) {
+int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const void* positions, int32_t positions_int64, const float* inv_freq, int32_t B,
+                      int32_t S, int32_t D, int32_t rope_dim, int32_t rope_start, int32_t norm_dim, int32_t interleaved, float rope_scale, float eps,
+                      void* workspace, size_t workspace_bytes, int32_t dtype, void* stream) {
   dsa::NormRopeParams p{};
-  if (!rows || !dy) return fail("null tensor pointer");
+  if (!q && !k) return fail("queries or keys must be given");
   if (fill_norm_rope(&p, positions, positions_int64, inv_freq, B, S, D, rope_dim, rope_start, norm_dim, interleaved, rope_scale, eps, dtype)) return 1;
-  if (fill_rope_side(&p.side[0], rows, D, norm_dim) || fill_rope_side(&p.side[1], nullptr, D, norm_dim)) return 1;
-  if (rows->slots || rows->split != D) return fail("the gradient is one contiguous tensor");
-  p.side[0].dy = dsa::RowView{dy, dy_stride_b, dy_stride_s, dy_stride_h};
-  if (d_weight || d_bias) {
-    if (!rows->norm) return fail("gradients of norm parameters need a norm");
-    if (!workspace || workspace_bytes < dsa::norm_rope_bwd_workspace_bytes(norm_dim)) return fail("workspace too small (see dsa_norm_rope_bwd_workspace_bytes)");
-    p.side[0].partials = static_cast<float*>(workspace);
+  const dsa_rope_grads* sides[2] = {q, k};
+  void* d_weight[2] = {nullptr, nullptr};
+  void* d_bias[2] = {nullptr, nullptr};
+  size_t used = 0;
+  for (int i = 0; i < 2; ++i) {
+    const dsa_rope_grads* g = sides[i];
+    if (fill_rope_side(&p.side[i], g ? &g->rows : nullptr, D, norm_dim)) return 1;
+    if (!g) continue;
+    if (!g->dy) return fail("null tensor pointer");
+    if (g->rows.slots || g->rows.split != D) return fail("the gradient is one contiguous tensor");
+    p.side[i].dy = dsa::RowView{g->dy, g->dy_stride_b, g->dy_stride_s, g->dy_stride_h};
+    if (g->d_weight || g->d_bias) {
+      if (!g->rows.norm) return fail("gradients of norm parameters need a norm");
+      const size_t need = dsa::norm_rope_bwd_workspace_bytes(norm_dim);
+      if (!workspace || workspace_bytes < used + need) return fail("workspace too small (see dsa_norm_rope_bwd_workspace_bytes)");
+      p.side[i].partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + used);
+      used += need;
+    }
+    d_weight[i] = g->d_weight;
+    d_bias[i] = g->d_bias;
   }
   int err = dsa::launch_norm_rope_bwd(p, d_weight, d_bias, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("norm_rope_bwd launch", err) : 0;

@@ -6,10 +6,13 @@
 //   backward: u = rot^T(dy); with n = (x - mean) rstd:  dweight = sum u n, dbias = sum u, g = u weight,
 //             dx = rstd (g - mean(g n) n [- mean(g)])
 //
-// Bound by memory: a row is read once and written once.  A group of 8, 16 or 32 lanes owns a row (16-byte units, all of them
-// in registers), a block owns a tile of tokens x heads; the cosines and sines of its tokens are made once per block, the
+// Bound by memory: a row is read once and written once.  A group of 8 lanes owns a row (above 576 dims: 16 lanes) and asks for all
+// of it at once, up to nine 16-byte units per lane, so that a warp has four rows on their way and no lane is without a unit for the
+// usual sizes (a warp per row left a quarter of its lanes idle at 576 dims and had one row on its way: 4096 tokens x 129 rows
+// of 576 dims 264 us).  A block owns a tile of tokens x heads; the cosines and sines of its tokens are made once per block, the
 // angle as an exact product reduced in 64 bits (a far position times a frequency has no fraction left in 32).
-// Everything is computed in fp32 and rounded once, on the store.
+// Everything is computed in fp32 and rounded once, on the store.  The gradient of rows without a norm is the forward with the angles
+// turned round.
 //
 // Rows that do not come in 16-byte units (odd sizes, offsets or strides) take the *_any kernels: a warp per row, one element
 // at a time, the same arithmetic.
@@ -28,15 +31,15 @@ constexpr int kThreads = 256;
 constexpr int kMaxPairs = 2048;      // (token, pair) angles a block keeps: 16 KB
 constexpr int kMaxNormDim = 1024;    // widest row of the 16-byte kernels
 
-// cos and sin of position * inv_freq, times the rotation's scale.
-__device__ __forceinline__ float2 turn_of(long long position, float inv_freq, float scale) {
+// cos and sin of position * inv_freq (p.back: of its negative), times the rotation's scale.
+__device__ __forceinline__ float2 turn_of(const NormRopeParams& p, long long position, float inv_freq) {
   const double angle = static_cast<double>(position) * static_cast<double>(inv_freq);
   const double turns = rint(angle * 0.15915494309189533577);          // 1 / 2 pi
   double r = fma(-turns, 6.283185307179586232, angle);                // 2 pi in two parts
   r = fma(-turns, 2.4492935982947064e-16, r);
   float s, c;
   sincosf(static_cast<float>(r), &s, &c);
-  return make_float2(c * scale, s * scale);
+  return make_float2(c * p.rope_scale, s * (p.back ? -p.rope_scale : p.rope_scale));
 }
 
 __device__ __forceinline__ long long position_of(const NormRopeParams& p, int token) {
@@ -90,20 +93,19 @@ __device__ __forceinline__ long long out_row(const RopeSide& sd, int token, int 
 }
 
 // The rotation of unit e0 .. e0 + 7 (dims relative to rope_start) of a row: v = this unit, o = its partner unit (halves only).
-// dir = +1 forward, -1 transposed.
-__device__ __forceinline__ void rotate8(float (&v)[8], const float (&o)[8], const float2* turns, int e0, int half, bool interleaved, float dir) {
+__device__ __forceinline__ void rotate8(float (&v)[8], const float (&o)[8], const float2* turns, int e0, int half, bool interleaved) {
   if (interleaved) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 t = turns[(e0 >> 1) + j];
-      const float a = v[2 * j], b = v[2 * j + 1], s = t.y * dir;
-      v[2 * j] = a * t.x - b * s;
-      v[2 * j + 1] = b * t.x + a * s;
+      const float a = v[2 * j], b = v[2 * j + 1];
+      v[2 * j] = a * t.x - b * t.y;
+      v[2 * j + 1] = b * t.x + a * t.y;
     }
   } else {
     const bool second = e0 >= half;
     const int i0 = second ? e0 - half : e0;
-    const float sign = second ? dir : -dir;
+    const float sign = second ? 1.f : -1.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float2 t = turns[i0 + j];
@@ -134,7 +136,7 @@ __device__ __forceinline__ Tile tile_of(const NormRopeParams& p, int block) {
 // forward, 16-byte units
 // -------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV>
-__global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   using namespace nr;
   extern __shared__ float2 turns[];                       // [tile_tokens][R / 2]
   __shared__ __align__(16) float sw[kMaxNormDim], sb[kMaxNormDim];
@@ -151,10 +153,12 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_co
     for (int i = 0; i < NV; ++i)
       if (lane + G * i < units) raw[i] = ld_stream(x + (lane + G * i) * 8);
   };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) raw[i] = make_uint4(0, 0, 0, 0);   // (units beyond the row stay zero)
   if (group < rows) fetch(group);   // the first row travels while the angles are made
   for (int i = tid; i < t.tokens * half; i += kThreads) {
     const int tk = i / half;
-    turns[i] = turn_of(position_of(p, t.token0 + tk), p.inv_freq[i - tk * half], p.rope_scale);
+    turns[i] = turn_of(p, position_of(p, t.token0 + tk), p.inv_freq[i - tk * half]);
   }
   if (sd.norm)
     for (int i = tid; i < p.norm_dim; i += kThreads) {
@@ -168,16 +172,7 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_co
     const int row = row0 + group;
     const bool live = row < rows;
     const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
-    float v[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (live && lane + G * i < units) unpack8<T>(raw[i], v[i]);
-      else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      }
-    }
-    if (row + kGroups < rows) fetch(row + kGroups);
+    if (row0 && live) fetch(row);
     float mean = 0.f, rstd = 1.f;
     if (sd.norm) {
       if (sd.norm == kNormLayer) {
@@ -185,8 +180,10 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if ((lane + G * i) * 8 < p.norm_dim) {
+            float v[8];
+            unpack8<T>(raw[i], v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[i][j];
+            for (int j = 0; j < 8; ++j) s += v[j];
           }
         mean = group_sum<G>(s) * p.inv_norm_dim;
       }
@@ -194,68 +191,75 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_kernel(const __grid_co
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if ((lane + G * i) * 8 < p.norm_dim) {
+          float v[8];
+          unpack8<T>(raw[i], v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) q += (v[i][j] - mean) * (v[i][j] - mean);
+          for (int j = 0; j < 8; ++j) q += (v[j] - mean) * (v[j] - mean);
         }
       rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int e = (lane + G * i) * 8;
-        if (e < p.norm_dim) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - mean) * rstd * sw[e + j] + sb[e + j];
-        }
-      }
     }
+    auto norm8 = [&](float (&v)[8], int e) {
+      if (sd.norm && e < p.norm_dim) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd * sw[e + j] + sb[e + j];
+      }
+    };
     const long long orow = live ? out_row(sd, token, head) : -1;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = (lane + G * i) * 8, r = e - p.rope_start;
-      if (!live || e >= p.D) continue;
-      if (r >= 0 && r < p.R) {
-        float o[8];
-        if (!p.interleaved) {   // the pair's other members lie in another lane's unit: read them again (the row is in L2) and norm them
+      float v[8], o[8];
+      unpack8<T>(raw[i], v);
+      norm8(v, e);
+      // (the same for all lanes: does the rotation touch these G units?)
+      if (G * i * 8 < p.rope_start + p.R && G * (i + 1) * 8 > p.rope_start) {
+        const bool turned = r >= 0 && r < p.R;
+        if (!p.interleaved) {   // the pairs' other members are another unit
           const int pe = r < half ? e + half : e - half;
-          unpack8<T>(__ldg(reinterpret_cast<const uint4*>(row_of<T>(sd.x, p.S, token, head) + pe)), o);
-          if (sd.norm && pe < p.norm_dim) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = (o[j] - mean) * rstd * sw[pe + j] + sb[pe + j];
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (p.partner_xor) {  // ... of the same turn of lane ^ partner_xor
+            w.x = __shfl_xor_sync(0xffffffffu, raw[i].x, p.partner_xor);
+            w.y = __shfl_xor_sync(0xffffffffu, raw[i].y, p.partner_xor);
+            w.z = __shfl_xor_sync(0xffffffffu, raw[i].z, p.partner_xor);
+            w.w = __shfl_xor_sync(0xffffffffu, raw[i].w, p.partner_xor);
+          } else if (live && turned) {   // ... read once more, from L2
+            w = __ldg(reinterpret_cast<const uint4*>(row_of<T>(sd.x, p.S, token, head) + pe));
           }
+          unpack8<T>(w, o);
+          if (turned) norm8(o, pe);
         }
-        rotate8(v[i], o, turns + tk * half, r, half, p.interleaved, 1.f);
+        if (turned) rotate8(v, o, turns + tk * half, r, half, p.interleaved);
       }
-      if (orow >= 0) {
+      if (orow >= 0 && e < p.D) {
         T* y = e < sd.split ? static_cast<T*>(sd.y) + orow * sd.split + e : static_cast<T*>(sd.y_tail) + orow * (p.D - sd.split) + (e - sd.split);
-        *reinterpret_cast<uint4*>(y) = pack8<T>(v[i]);
+        *reinterpret_cast<uint4*>(y) = pack8<T>(v);
       }
     }
   }
 }
 
 // -------------------------------------------------------------------------------------------------
-// backward of one side, 16-byte units.  With a norm every block leaves the sums of its rows for dweight and dbias in its own
+// backward of one side with a norm, 16-byte units.  Every block leaves the sums of its rows for dweight and dbias in its own
 // line of the workspace (norm_rope_param_grad_kernel adds the lines up in a fixed order).
 // -------------------------------------------------------------------------------------------------
-template <typename T, int G, int NV, bool kNorm>
+template <typename T, int G, int NV>
 __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
   using namespace nr;
   extern __shared__ float2 turns[];
-  __shared__ __align__(16) float sw[kNorm ? kMaxNormDim : 1], sdw[kNorm ? kMaxNormDim : 1], sdb[kNorm ? kMaxNormDim : 1];
+  __shared__ __align__(16) float sw[kMaxNormDim], sdw[kMaxNormDim], sdb[kMaxNormDim];
   const RopeSide& sd = p.side[0];
   const int tid = threadIdx.x, lane = tid % G, group = tid / G;
   constexpr int kGroups = kThreads / G;
   const int units = p.D >> 3, half = p.R >> 1;
-  float dw[kNorm ? NV : 1][8], db[kNorm ? NV : 1][8];
-  if constexpr (kNorm) {
+  float dw[NV][8], db[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f;
-    }
-    for (int i = tid; i < p.norm_dim; i += kThreads) {
-      sw[i] = sd.weight ? param_at<T>(sd.weight, sd.param_fp32, i) : 1.f;
-      sdw[i] = sdb[i] = 0.f;
-    }
+    for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f;
+  }
+  for (int i = tid; i < p.norm_dim; i += kThreads) {
+    sw[i] = sd.weight ? param_at<T>(sd.weight, sd.param_fp32, i) : 1.f;
+    sdw[i] = sdb[i] = 0.f;
   }
   for (int tile = blockIdx.x; tile < sd.blocks; tile += gridDim.x) {
     const Tile t = tile_of(p, tile);
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
     __syncthreads();   // the last tile's angles have been used
     for (int i = tid; i < t.tokens * half; i += kThreads) {
       const int tk = i / half;
-      turns[i] = turn_of(position_of(p, t.token0 + tk), p.inv_freq[i - tk * half], p.rope_scale);
+      turns[i] = turn_of(p, position_of(p, t.token0 + tk), p.inv_freq[i - tk * half]);
     }
     __syncthreads();
     for (int row0 = 0; row0 < rows; row0 += kGroups) {
@@ -271,17 +275,16 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
       const bool live = row < rows;
       const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
       const T* dy = row_of<T>(sd.dy, p.S, token, head);
-      float v[NV][8], x[kNorm ? NV : 1][8];
+      float v[NV][8], x[NV][8];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         uint4 w = make_uint4(0, 0, 0, 0), wx = w;
         if (live && lane + G * i < units) {
           w = ld_stream(dy + (lane + G * i) * 8);
-          if constexpr (kNorm)
-            if ((lane + G * i) * 8 < p.norm_dim) wx = ld_stream(row_of<T>(sd.x, p.S, token, head) + (lane + G * i) * 8);
+          if ((lane + G * i) * 8 < p.norm_dim) wx = ld_stream(row_of<T>(sd.x, p.S, token, head) + (lane + G * i) * 8);
         }
         unpack8<T>(w, v[i]);
-        if constexpr (kNorm) unpack8<T>(wx, x[i]);
+        unpack8<T>(wx, x[i]);
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -289,53 +292,51 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
         if (live && e < p.D && r >= 0 && r < p.R) {
           float o[8];
           if (!p.interleaved) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(dy + (r < half ? e + half : e - half))), o);
-          rotate8(v[i], o, turns + tk * half, r, half, p.interleaved, -1.f);
+          rotate8(v[i], o, turns + tk * half, r, half, p.interleaved);
         }
       }
-      if constexpr (kNorm) {
-        float mean = 0.f;
-        if (sd.norm == kNormLayer) {
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += x[i][j];   // (units beyond norm_dim hold zeros)
-          }
-          mean = group_sum<G>(s) * p.inv_norm_dim;
-        }
-        float q = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if ((lane + G * i) * 8 < p.norm_dim) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { x[i][j] -= mean; q += x[i][j] * x[i][j]; }
-          }
-        const float rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
-        float gn = 0.f, gs = 0.f;
+      float mean = 0.f;
+      if (sd.norm == kNormLayer) {
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int e = (lane + G * i) * 8;
-          if (e < p.norm_dim) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              x[i][j] *= rstd;
-              dw[i][j] += v[i][j] * x[i][j];
-              db[i][j] += v[i][j];
-              v[i][j] *= sw[e + j];
-              gn += v[i][j] * x[i][j];
-              gs += v[i][j];
-            }
+          for (int j = 0; j < 8; ++j) s += x[i][j];   // (units beyond norm_dim hold zeros)
+        }
+        mean = group_sum<G>(s) * p.inv_norm_dim;
+      }
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { x[i][j] -= mean; q += x[i][j] * x[i][j]; }
+        }
+      const float rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
+      float gn = 0.f, gs = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = (lane + G * i) * 8;
+        if (e < p.norm_dim) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[i][j] *= rstd;
+            dw[i][j] += v[i][j] * x[i][j];
+            db[i][j] += v[i][j];
+            v[i][j] *= sw[e + j];
+            gn += v[i][j] * x[i][j];
+            gs += v[i][j];
           }
         }
-        gn = group_sum<G>(gn) * p.inv_norm_dim;
-        gs = sd.norm == kNormLayer ? group_sum<G>(gs) * p.inv_norm_dim : 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if ((lane + G * i) * 8 < p.norm_dim) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = rstd * (v[i][j] - gn * x[i][j] - gs);
-          }
       }
+      gn = group_sum<G>(gn) * p.inv_norm_dim;
+      gs = sd.norm == kNormLayer ? group_sum<G>(gs) * p.inv_norm_dim : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((lane + G * i) * 8 < p.norm_dim) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = rstd * (v[i][j] - gn * x[i][j] - gs);
+        }
       if (live) {
         T* dx = static_cast<T*>(sd.y) + (static_cast<long long>(token) * sd.H + head) * p.D;
 #pragma unroll
@@ -344,26 +345,24 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
       }
     }
   }
-  if constexpr (kNorm) {
-    if (!sd.partials) return;
-    // the groups of the block add their sums one after the other: the same order in every run
-    for (int turn = 0; turn < kGroups; ++turn) {
-      __syncthreads();
-      if (group == turn) {
+  if (!sd.partials) return;
+  // the groups of the block add their sums one after the other: the same order in every run
+  for (int turn = 0; turn < kGroups; ++turn) {
+    __syncthreads();
+    if (group == turn) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int e = (lane + G * i) * 8;
-          if (e < p.norm_dim) {
+      for (int i = 0; i < NV; ++i) {
+        const int e = (lane + G * i) * 8;
+        if (e < p.norm_dim) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { sdw[e + j] += dw[i][j]; sdb[e + j] += db[i][j]; }
-          }
+          for (int j = 0; j < 8; ++j) { sdw[e + j] += dw[i][j]; sdb[e + j] += db[i][j]; }
         }
       }
     }
-    __syncthreads();
-    float* line = sd.partials + static_cast<long long>(blockIdx.x) * 2 * p.norm_dim;
-    for (int i = tid; i < p.norm_dim; i += kThreads) { line[i] = sdw[i]; line[p.norm_dim + i] = sdb[i]; }
   }
+  __syncthreads();
+  float* line = sd.partials + static_cast<long long>(blockIdx.x) * 2 * p.norm_dim;
+  for (int i = tid; i < p.norm_dim; i += kThreads) { line[i] = sdw[i]; line[p.norm_dim + i] = sdb[i]; }
 }
 
 // dweight and dbias from the blocks' lines: a block takes 32 columns of the 2 * norm_dim, its warps every eighth line.
@@ -409,16 +408,16 @@ __device__ __forceinline__ void any_stats(const NormRopeParams& p, const RopeSid
   *rstd = rsqrtf(group_sum<32>(q) * p.inv_norm_dim + p.eps);
 }
 
-// Element e of the rotated row (dir = -1: rotated back) whose elements `at` gives.
+// Element e of the rotated row whose elements `at` gives.
 template <typename At>
-__device__ __forceinline__ float any_rotated(const NormRopeParams& p, long long position, int e, float dir, At at) {
+__device__ __forceinline__ float any_rotated(const NormRopeParams& p, long long position, int e, At at) {
   const int d = e - p.rope_start, half = p.R >> 1;
   if (d < 0 || d >= p.R) return at(e);
   const bool second = p.interleaved ? (d & 1) != 0 : d >= half;
   const int pair = p.interleaved ? d >> 1 : (second ? d - half : d);
   const int partner = p.interleaved ? p.rope_start + (d ^ 1) : (second ? e - half : e + half);
-  const float2 t = turn_of(position, p.inv_freq[pair], p.rope_scale);
-  return at(e) * t.x + at(partner) * (second ? dir * t.y : -dir * t.y);
+  const float2 t = turn_of(p, position, p.inv_freq[pair]);
+  return at(e) * t.x + at(partner) * (second ? t.y : -t.y);
 }
 
 template <typename T, bool kBack>
@@ -439,7 +438,7 @@ __device__ __forceinline__ void any_row(const NormRopeParams& p, const RopeSide&
     };
     for (int e = lane; e < p.D; e += 32) {
       T* y = e < sd.split ? static_cast<T*>(sd.y) + orow * sd.split + e : static_cast<T*>(sd.y_tail) + orow * (p.D - sd.split) + (e - sd.split);
-      *y = static_cast<T>(any_rotated(p, position, e, 1.f, normed));
+      *y = static_cast<T>(any_rotated(p, position, e, normed));
     }
   } else {
     const T* dy = row_of<T>(sd.dy, p.S, token, head);
@@ -447,7 +446,7 @@ __device__ __forceinline__ void any_row(const NormRopeParams& p, const RopeSide&
     float gn = 0.f, gs = 0.f;
     if (sd.norm) {
       for (int e = lane; e < n; e += 32) {
-        const float u = any_rotated(p, position, e, -1.f, grad) * weight(e);
+        const float u = any_rotated(p, position, e, grad) * weight(e);
         gn += u * (static_cast<float>(x[e]) - mean) * rstd;
         gs += u;
       }
@@ -456,7 +455,7 @@ __device__ __forceinline__ void any_row(const NormRopeParams& p, const RopeSide&
     }
     T* dx = static_cast<T*>(sd.y) + r * p.D;
     for (int e = lane; e < p.D; e += 32) {
-      float u = any_rotated(p, position, e, -1.f, grad);
+      float u = any_rotated(p, position, e, grad);
       if (sd.norm && e < n) u = rstd * (u * weight(e) - gn * (static_cast<float>(x[e]) - mean) * rstd - gs);
       dx[e] = static_cast<T>(u);
     }
@@ -495,7 +494,7 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_any_kernel(const __gri
           any_stats(p, sd, x, lane, &mean, &rstd);
           const long long position = position_of(p, token);
           for (int e = lane; e < p.norm_dim; e += 32) {
-            const float u = any_rotated(p, position, e, -1.f, [&](int i) { return static_cast<float>(dy[i]); });
+            const float u = any_rotated(p, position, e, [&](int i) { return static_cast<float>(dy[i]); });
             line[e] += u * (static_cast<float>(x[e]) - mean) * rstd;
             line[p.norm_dim + e] += u;
           }
@@ -549,25 +548,29 @@ int tile_smem(const NormRopeParams& p) {
 }
 
 template <typename T, int G, int NV>
-int forward(const NormRopeParams& p, cudaStream_t stream) {
+int forward(NormRopeParams p, cudaStream_t stream) {
+  // Halves: does a unit's partner sit in the same turn of another lane of its group, at a fixed lane distance?
+  const int d = p.R / 16;
+  p.partner_xor = !p.interleaved && 2 * d <= G && (d & (d - 1)) == 0 && p.rope_start % (16 * d) == 0 ? d : 0;
   norm_rope_kernel<T, G, NV><<<p.side[0].blocks + p.side[1].blocks, nr::kThreads, tile_smem(p), stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T, int G, int NV>
 int backward(const NormRopeParams& p, int grid, cudaStream_t stream) {
-  if (p.side[0].norm) norm_rope_bwd_kernel<T, G, NV, true><<<grid, nr::kThreads, tile_smem(p), stream>>>(p);
-  else norm_rope_bwd_kernel<T, G, NV, false><<<grid, nr::kThreads, tile_smem(p), stream>>>(p);
+  norm_rope_bwd_kernel<T, G, NV><<<grid, nr::kThreads, tile_smem(p), stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T>
 int forward_units(const NormRopeParams& p, cudaStream_t stream) {
   if (p.D <= 64) return forward<T, 8, 1>(p, stream);
-  if (p.D <= 128) return forward<T, 16, 1>(p, stream);
-  if (p.D <= 256) return forward<T, 32, 1>(p, stream);
-  if (p.D <= 512) return forward<T, 32, 2>(p, stream);
-  if (p.D <= 768) return forward<T, 32, 3>(p, stream);
-  return forward<T, 32, 4>(p, stream);
+  if (p.D <= 128) return forward<T, 8, 2>(p, stream);
+  if (p.D <= 192) return forward<T, 8, 3>(p, stream);
+  if (p.D <= 256) return forward<T, 8, 4>(p, stream);
+  if (p.D <= 512) return forward<T, 8, 8>(p, stream);
+  if (p.D <= 576) return forward<T, 8, 9>(p, stream);
+  return forward<T, 16, 8>(p, stream);
 }
+// (the sums for dweight and dbias take 16 registers per unit of a lane: up to 32 lanes per row)
 template <typename T>
 int backward_units(const NormRopeParams& p, int grid, cudaStream_t stream) {
   if (p.D <= 64) return backward<T, 8, 1>(p, grid, stream);
@@ -602,28 +605,49 @@ size_t norm_rope_bwd_workspace_bytes(int norm_dim) {
   return static_cast<size_t>(norm_lines(sms)) * 2 * norm_dim * sizeof(float);
 }
 
-// p.side[0]: x (norm only), dy, y = dx, partials = workspace when dweight or dbias is asked for.
-int launch_norm_rope_bwd(NormRopeParams p, void* d_weight, void* d_bias, bool bf16, cudaStream_t stream) {
+// Sides with x (norm only), dy, y = dx; d_weight / d_bias with the side's partials in the workspace, or null.
+int launch_norm_rope_bwd(NormRopeParams p, void* const d_weight[2], void* const d_bias[2], bool bf16, cudaStream_t stream) {
   int dev = 0, sms = 0;
   cudaError_t e = current_device_sms(&dev, &sms);
   if (e != cudaSuccess) return static_cast<int>(e);
-  int grid, err;
-  if (!in_units(p)) {
-    const long long want = (static_cast<long long>(p.tokens) * p.side[0].H + 7) / 8;
-    grid = static_cast<int>(want < norm_lines(sms) ? want : norm_lines(sms));
-    if (bf16) norm_rope_any_kernel<__nv_bfloat16, true><<<grid, nr::kThreads, 0, stream>>>(p);
-    else norm_rope_any_kernel<__half, true><<<grid, nr::kThreads, 0, stream>>>(p);
-    err = static_cast<int>(cudaGetLastError());
-  } else {
-    tiles(&p, sms);
-    grid = p.side[0].norm && p.side[0].blocks > norm_lines(sms) ? norm_lines(sms) : p.side[0].blocks;
-    err = bf16 ? backward_units<__nv_bfloat16>(p, grid, stream) : backward_units<__half>(p, grid, stream);
+  p.back = 1;
+  // sides without a norm: the forward with the angles turned round, both in one launch
+  NormRopeParams turned = p;
+  for (RopeSide& sd : turned.side) {
+    if (sd.norm) sd.H = 0;
+    sd.x = sd.dy;
   }
-  if (err || !p.side[0].partials) return err;
-  const int cols = (2 * p.norm_dim + 31) / 32;
-  if (bf16) norm_rope_param_grad_kernel<__nv_bfloat16><<<cols, 256, 0, stream>>>(p.side[0].partials, grid, p.norm_dim, d_weight, d_bias, p.side[0].param_fp32);
-  else norm_rope_param_grad_kernel<__half><<<cols, 256, 0, stream>>>(p.side[0].partials, grid, p.norm_dim, d_weight, d_bias, p.side[0].param_fp32);
-  return static_cast<int>(cudaGetLastError());
+  if (turned.side[0].H || turned.side[1].H) {
+    const int err = launch_norm_rope(turned, bf16, stream);
+    if (err) return err;
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (!p.side[i].H || !p.side[i].norm) continue;
+    NormRopeParams one = p;
+    one.side[0] = p.side[i];
+    one.side[1].H = 0;
+    int grid, err;
+    if (!in_units(one)) {
+      const long long want = (static_cast<long long>(one.tokens) * one.side[0].H + 7) / 8;
+      grid = static_cast<int>(want < norm_lines(sms) ? want : norm_lines(sms));
+      if (bf16) norm_rope_any_kernel<__nv_bfloat16, true><<<grid, nr::kThreads, 0, stream>>>(one);
+      else norm_rope_any_kernel<__half, true><<<grid, nr::kThreads, 0, stream>>>(one);
+      err = static_cast<int>(cudaGetLastError());
+    } else {
+      tiles(&one, sms);
+      grid = one.side[0].blocks > norm_lines(sms) ? norm_lines(sms) : one.side[0].blocks;
+      err = bf16 ? backward_units<__nv_bfloat16>(one, grid, stream) : backward_units<__half>(one, grid, stream);
+    }
+    if (err) return err;
+    if (!one.side[0].partials) continue;
+    const int cols = (2 * p.norm_dim + 31) / 32;
+    if (bf16)
+      norm_rope_param_grad_kernel<__nv_bfloat16><<<cols, 256, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
+    else
+      norm_rope_param_grad_kernel<__half><<<cols, 256, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
+    if ((err = static_cast<int>(cudaGetLastError()))) return err;
+  }
+  return 0;
 }
 
 }  // namespace dsa

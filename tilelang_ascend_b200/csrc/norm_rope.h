@@ -42,10 +42,12 @@ struct NormRopeParams {
   const float* inv_freq;  // [R / 2]
   int tokens, S, D, R, rope_start, norm_dim, interleaved;
   float rope_scale, eps, inv_norm_dim;
+  int back;               // 1: the transposed rotation
+  int partner_xor;        // set by the launcher
 };
 
 int launch_norm_rope(NormRopeParams p, bool bf16, cudaStream_t stream);
 size_t norm_rope_bwd_workspace_bytes(int norm_dim);
-int launch_norm_rope_bwd(NormRopeParams p, void* d_weight, void* d_bias, bool bf16, cudaStream_t stream);
+int launch_norm_rope_bwd(NormRopeParams p, void* const d_weight[2], void* const d_bias[2], bool bf16, cudaStream_t stream);
 
 }  // namespace dsa

@@ -13,89 +13,110 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .adapter import check_inputs, current_stream, dtype_code, ptr
+from .adapter import check_inputs, dtype_code, on_device, ptr, raw_stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _TEACHERS = {"weights": 0, "logits": 1}
 _OVER = {"list": 0, "row": 1}
 
 
-class _Rows:
-    """Checked arguments of a distillation: [..., V] student rows, [..., K] teacher entries."""
+def _check_rows(student, teacher, indices, teacher_kind, over, temperature) -> torch.device:
+    """Arguments of a distillation: [..., V] student rows, [..., K] teacher entries."""
+    if teacher_kind not in _TEACHERS:
+        raise ValueError(f"teacher_kind must be 'weights' or 'logits', got {teacher_kind!r}")
+    if over not in _OVER:
+        raise ValueError(f"over must be 'list' or 'row', got {over!r}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    for t, name in ((student, "student"), (teacher, "teacher")):
+        if not isinstance(t, torch.Tensor) or t.dim() < 1:
+            raise ValueError(f"{name} must be a tensor of rows")
+        if t.dtype not in _TYPES:
+            raise ValueError(f"Input tensor {name} has dtype {t.dtype}, expected bfloat16, float16 or float32")
+    V, K, dev = student.shape[-1], teacher.shape[-1], student.device
+    if teacher.shape[:-1] != student.shape[:-1]:
+        raise ValueError(f"student {tuple(student.shape)} and teacher {tuple(teacher.shape)} must have the same rows")
+    if V < 1 or K < 1:
+        raise ValueError("rows need at least one column and one entry")
+    if not teacher.is_contiguous():
+        raise ValueError("Input tensor teacher must be contiguous")
+    if indices is None:
+        if K != V:
+            raise ValueError(f"without indices the teacher has one entry per column (got {K} for {V})")
+    else:
+        if indices.dtype != torch.int32:
+            raise ValueError(f"Input tensor indices has dtype {indices.dtype}, expected torch.int32")
+        if indices.shape != teacher.shape or not indices.is_contiguous():
+            raise ValueError(f"indices must be contiguous {tuple(teacher.shape)}, got {tuple(indices.shape)}")
+    _row_stride(student)
+    for t, name in ((teacher, "teacher"), (indices, "indices")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"Input tensor {name} is on {t.device}, expected {dev}")
+    return dev
 
-    def __init__(self, student, teacher, indices, teacher_kind, over, temperature):
-        if teacher_kind not in _TEACHERS:
-            raise ValueError(f"teacher_kind must be 'weights' or 'logits', got {teacher_kind!r}")
-        if over not in _OVER:
-            raise ValueError(f"over must be 'list' or 'row', got {over!r}")
-        self.temperature = float(temperature)
-        if not 0.0 < self.temperature < float("inf"):
-            raise ValueError(f"temperature must be positive and finite, got {temperature}")
-        for t, name in ((student, "student"), (teacher, "teacher")):
-            if not isinstance(t, torch.Tensor) or t.dim() < 1:
-                raise ValueError(f"{name} must be a tensor of rows")
-            if t.dtype not in _TYPES:
-                raise ValueError(f"Input tensor {name} has dtype {t.dtype}, expected bfloat16, float16 or float32")
-        self.lead, self.V, self.K = student.shape[:-1], student.shape[-1], teacher.shape[-1]
-        if teacher.shape[:-1] != self.lead:
-            raise ValueError(f"student {tuple(student.shape)} and teacher {tuple(teacher.shape)} must have the same rows")
-        if self.V < 1 or self.K < 1:
-            raise ValueError("rows need at least one column and one entry")
-        if not teacher.is_contiguous():
-            raise ValueError("Input tensor teacher must be contiguous")
-        if indices is None:
-            if self.K != self.V:
-                raise ValueError(f"without indices the teacher has one entry per column (got {self.K} for {self.V})")
-        else:
-            if indices.dtype != torch.int32:
-                raise ValueError(f"Input tensor indices has dtype {indices.dtype}, expected torch.int32")
-            if indices.shape != teacher.shape or not indices.is_contiguous():
-                raise ValueError(f"indices must be contiguous {tuple(teacher.shape)}, got {tuple(indices.shape)}")
-        try:
-            rows = student.view(-1, self.V) if student.numel() else student
-        except RuntimeError:
-            rows = None
-        if rows is None or (student.numel() and self.V > 1 and rows.stride(1) != 1):
-            raise ValueError("student must have unit inner stride and evenly spaced rows")
-        self.rows = student.numel() // self.V
-        self.row_stride = rows.stride(0) if student.numel() else self.V
-        self.dev = student.device
-        for t, name in ((teacher, "teacher"), (indices, "indices")):
-            if t is not None and t.device != self.dev:
-                raise ValueError(f"Input tensor {name} is on {t.device}, expected {self.dev}")
-        self.head = (ptr(student), _TYPES[student.dtype], self.row_stride, ptr(teacher), _TYPES[teacher.dtype], ptr(indices))
-        self.tail = (self.rows, self.V, self.K, _OVER[over], _TEACHERS[teacher_kind], self.temperature)
 
-    def require_cuda(self) -> None:
-        if self.dev.type != "cuda":
-            raise ValueError(f"kernels run on CUDA tensors only (got device {self.dev}); there is no CPU path")
+def _row_stride(student) -> int:
+    """Elements between a student's rows."""
+    if student.is_contiguous():
+        return student.shape[-1]
+    try:
+        rows = student.view(-1, student.shape[-1])
+    except RuntimeError:
+        rows = None
+    if rows is None or (rows.stride(1) != 1 and rows.shape[1] > 1):
+        raise ValueError("student must have unit inner stride and evenly spaced rows")
+    return rows.stride(0)
+
+
+def _head(student, teacher, indices):
+    return student.data_ptr(), _TYPES[student.dtype], _row_stride(student), teacher.data_ptr(), _TYPES[teacher.dtype], ptr(indices)
+
+
+def _tail(student, teacher, teacher_kind, over, temperature):
+    V = student.shape[-1]
+    return student.numel() // V, V, teacher.shape[-1], _OVER[over], _TEACHERS[teacher_kind], temperature
+
+
+def _require_cuda(dev) -> None:
+    if dev.type != "cuda":
+        raise ValueError(f"kernels run on CUDA tensors only (got device {dev}); there is no CPU path")
 
 
 def topk_distillation_raw(student, teacher, indices=None, *, teacher_kind: str = "weights", over: str = "list",
                           temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(loss [...], stats [rows, 4]) of :func:`topk_distillation`; the backward takes the stats."""
-    r = _Rows(student, teacher, indices, teacher_kind, over, temperature)
-    r.require_cuda()
-    loss = torch.empty(r.lead, dtype=torch.float32, device=r.dev)
-    stats = torch.empty((r.rows, 4), dtype=torch.float32, device=r.dev)
-    if r.rows:
-        with torch.cuda.device(r.dev):
-            _lib.check(_lib.load().dsa_topk_distillation(*r.head, ptr(loss), ptr(stats), *r.tail, current_stream(r.dev)))
+    temperature = float(temperature)
+    dev = _check_rows(student, teacher, indices, teacher_kind, over, temperature)
+    _require_cuda(dev)
+    tail = _tail(student, teacher, teacher_kind, over, temperature)
+    loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=dev)
+    stats = torch.empty((tail[0], 4), dtype=torch.float32, device=dev)
+    if tail[0]:
+        with on_device(dev):
+            _lib.check(_lib.load().dsa_topk_distillation(*_head(student, teacher, indices), loss.data_ptr(), stats.data_ptr(), *tail, raw_stream(dev)))
     return loss, stats
+
+
+def _gradient(student, teacher, indices, stats, grad, teacher_kind, over, temperature):
+    """Gradient of checked rows."""
+    dev, tail = student.device, _tail(student, teacher, teacher_kind, over, temperature)
+    d_student = torch.empty(student.shape, dtype=student.dtype, device=dev)
+    if tail[0]:
+        with on_device(dev):
+            _lib.check(_lib.load().dsa_topk_distillation_bwd(*_head(student, teacher, indices), stats.data_ptr(), grad.data_ptr(), d_student.data_ptr(), *tail,
+                                                             raw_stream(dev)))
+    return d_student
 
 
 def topk_distillation_bwd_raw(student, teacher, indices, stats, grad, *, teacher_kind: str = "weights", over: str = "list", temperature: float = 1.0):
     """Gradient of the student's rows (contiguous, the student's dtype) for ``grad`` [...] of the losses."""
-    r = _Rows(student, teacher, indices, teacher_kind, over, temperature)
-    for t, name, shape in ((stats, "stats", (r.rows, 4)), (grad, "grad", tuple(r.lead))):
-        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != r.dev:
-            raise ValueError(f"{name} must be contiguous float32 {shape} on {r.dev}")
-    r.require_cuda()
-    d_student = torch.empty(student.shape, dtype=student.dtype, device=r.dev)
-    if r.rows:
-        with torch.cuda.device(r.dev):
-            _lib.check(_lib.load().dsa_topk_distillation_bwd(*r.head, ptr(stats), ptr(grad), ptr(d_student), *r.tail, current_stream(r.dev)))
-    return d_student
+    temperature = float(temperature)
+    dev = _check_rows(student, teacher, indices, teacher_kind, over, temperature)
+    for t, name, shape in ((stats, "stats", (student.numel() // student.shape[-1], 4)), (grad, "grad", student.shape[:-1])):
+        if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} must be contiguous float32 {tuple(shape)} on {dev}")
+    _require_cuda(dev)
+    return _gradient(student, teacher, indices, stats, grad, teacher_kind, over, temperature)
 
 
 class TopkDistillationFunction(torch.autograd.Function):
@@ -103,18 +124,15 @@ class TopkDistillationFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, student, teacher, indices, teacher_kind, over, temperature):
-        ctx.how = dict(teacher_kind=teacher_kind, over=over, temperature=temperature)
-        loss, stats = topk_distillation_raw(student, teacher, indices, **ctx.how)
+        loss, stats = topk_distillation_raw(student, teacher, indices, teacher_kind=teacher_kind, over=over, temperature=temperature)
+        ctx.how = teacher_kind, over, float(temperature)
         ctx.save_for_backward(student, teacher, indices, stats)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        student, teacher, indices, stats = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            return (None,) * 6
-        return (topk_distillation_bwd_raw(student, teacher, indices, stats, grad.contiguous(), **ctx.how),) + (None,) * 5
+        return _gradient(*ctx.saved_tensors, grad.contiguous(), *ctx.how), None, None, None, None, None
 
 
 def topk_distillation(student, teacher, indices: Optional[torch.Tensor] = None, *, teacher_kind: str = "weights", over: str = "list",
@@ -155,15 +173,21 @@ def lightning_indexer_bwd_raw(query, key, weights, indices, d_values):
     """Gradients of the indexer's scores at listed keys: (d_query in the query's dtype, d_key fp32, d_weights fp32) for ``d_values``
     [B,S1,1,K] fp32.  Entries of ``indices`` outside [0, S2) take no part, whatever d_values holds there.  relu'(0) = 0.  The key
     gradient is summed with fp32 atomics: its last bits depend on their order."""
-    dev = _check_indexer(query, key, weights, indices, [(d_values, "d_values")])
+    _check_indexer(query, key, weights, indices, [(d_values, "d_values")])
+    return _indexer_gradients(query, key, weights, indices, d_values)
+
+
+def _indexer_gradients(query, key, weights, indices, d_values):
+    """The same for checked tensors."""
     B, S1, N1, D = query.shape
+    dev = query.device
     d_query, d_weights = torch.empty_like(query), torch.empty_like(weights)
     d_key = torch.zeros(key.shape, dtype=torch.float32, device=dev)
     if B * S1:
-        with torch.cuda.device(dev):
+        with on_device(dev):
             _lib.check(_lib.load().dsa_lightning_indexer_bwd(
-                ptr(query), ptr(key), ptr(weights), ptr(indices), ptr(d_values), ptr(d_query), ptr(d_key), ptr(d_weights), B, S1, key.shape[1], N1, D,
-                indices.shape[3], dtype_code(query.dtype), current_stream(dev)))
+                query.data_ptr(), key.data_ptr(), weights.data_ptr(), indices.data_ptr(), d_values.data_ptr(), d_query.data_ptr(), d_key.data_ptr(),
+                d_weights.data_ptr(), B, S1, key.shape[1], N1, D, indices.shape[3], dtype_code(query.dtype), raw_stream(dev)))
     return d_query, d_key, d_weights
 
 
@@ -173,8 +197,8 @@ class LightningIndexerDistillationFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, weights, indices, values, teacher, teacher_kind, temperature):
         _check_indexer(query, key, weights, indices, [(values, "values"), (teacher, "teacher")])
-        ctx.how = dict(teacher_kind=teacher_kind, temperature=temperature)
-        loss, stats = topk_distillation_raw(values, teacher, None, **ctx.how)
+        loss, stats = topk_distillation_raw(values, teacher, None, teacher_kind=teacher_kind, temperature=temperature)
+        ctx.how = teacher_kind, "list", float(temperature)
         ctx.save_for_backward(query, key, weights, indices, values, teacher, stats)
         return loss.squeeze(2)
 
@@ -182,8 +206,8 @@ class LightningIndexerDistillationFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         query, key, weights, indices, values, teacher, stats = ctx.saved_tensors
-        d_values = topk_distillation_bwd_raw(values, teacher, None, stats, grad.contiguous().unsqueeze(2), **ctx.how)
-        d_query, d_key, d_weights = lightning_indexer_bwd_raw(query, key, weights, indices, d_values)
+        d_values = _gradient(values, teacher, None, stats, grad.contiguous(), *ctx.how)
+        d_query, d_key, d_weights = _indexer_gradients(query, key, weights, indices, d_values)
         return d_query, d_key.to(key.dtype), d_weights, None, None, None, None, None
 
 

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .adapter import check_inputs, current_stream, dtype_code, ptr, torch_dtype
+from .adapter import check_inputs, current_stream, dtype_code, on_device, ptr, raw_stream, torch_dtype
 
 
 def _check_distinct_indices(indices: torch.Tensor, S_kv: int) -> None:
@@ -371,8 +371,8 @@ def sparse_mla_key_weights(q, kv, indices, lse, *, sm_scale: Optional[float] = N
     dev = check_inputs([q, kv, indices, lse], [None, q.dtype, torch.int32, torch.float32], ["q", "kv", "indices", "lse"])
     weights = torch.empty((B, S, 1, topk), dtype=torch.float32, device=dev)
     if B * S:
-        with torch.cuda.device(dev):
+        with on_device(dev):
             _lib.check(_lib.load().dsa_sparse_mla_key_weights(
                 ptr(q), ptr(kv), ptr(indices), ptr(lse), ptr(weights), B, S, S_kv, H, D, topk, float(D ** -0.5 if sm_scale is None else sm_scale),
-                S_kv - S if q_start_index_s is None else int(q_start_index_s), 1, code, current_stream(dev)))
+                S_kv - S if q_start_index_s is None else int(q_start_index_s), 1, code, raw_stream(dev)))
     return weights
