@@ -6,9 +6,12 @@
 //     loss = sum_j p_j (log p_j - log s_j)             d student_c = g / T (s_c - sum of the p_j at c)
 //   A row without participating entries, or whose teacher holds nothing there, has loss 0 and gradient 0.
 //
-// Bound by memory: the forward reads the row once (online maximum and sum when it is normalised over the whole row), the backward reads it
-// once more and writes the gradient.  The logarithm of a probability is taken as a difference to the row's maximum; all sums in fp32.  Backward with indices: a block owns 8192 columns of a row, adds the listed
-// entries of its columns up in shared memory (a column may be listed more than once) and then streams the columns.
+// Bound by memory: the forward reads the row and the list once -- every thread carries running maxima and the sums relative to
+// them (softmax normaliser S, teacher weight W, A = sum w (log w - z)), joined over the block at the end: loss = A / W - log W + log S --,
+// the backward reads them once more and writes the gradient.  Everything is taken relative to the maxima, so rows far from zero keep
+// their digits; all sums in fp32.  (Entries kept in registers and three passes over them: 4096 lists of 2048 forward 87 us; exact
+// logarithms and divisions per entry were half of that.)  Backward with indices: a block owns 8192 columns of a row, asks for them,
+// adds the listed entries of its columns up in shared memory meanwhile (a column may be listed more than once) and writes the columns.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -21,13 +24,21 @@
 namespace dsa {
 
 namespace dt {
-constexpr float kLowest = -3.402823466e38f;
-constexpr int kChunk = 8192;   // columns of a backward block: 32 KB of sums
+constexpr float kLowest = -3.402823466e38f, kLn2 = 0.6931471805599453f;
+constexpr int kChunk = 8192;         // columns of a backward block with indices: 32 KB of sums
+constexpr int kListedThreads = 512;
+constexpr int kPerThread = kChunk / kListedThreads;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// ln of a weight: lg2 within 2^-22 (relative, or absolute next to 1)
+__device__ __forceinline__ float ln_of(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y * kLn2;
 }
 // exp((x - m) / T) with c = log2(e) / T: the difference is taken before anything is rounded, so rows far from zero keep their
 // digits; x = -inf gives 0 for any finite m
@@ -35,70 +46,114 @@ __device__ __forceinline__ float exp_from(float x, float m, float c) { return ex
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v) { return static_cast<float>(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v) { return static_cast<T>(v); }
 
+// Four consecutive values (at a multiple of four elements).
 template <typename T>
-struct Vec {
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 w = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+  } else {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = to_f(e[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint2 w;
+    T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<uint2*>(p) = w;
+  }
+}
+template <typename T>
+struct Vec {   // 16 bytes
   static constexpr int kN = 16 / sizeof(T);
   uint4 raw;
   __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ float get(int i) const { return to_f(reinterpret_cast<const T*>(&raw)[i]); }
-  __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f<T>(v); }
+  __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = static_cast<T>(v); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
 };
 
+__device__ __forceinline__ void teacher4(const DistillParams& p, int64_t i, float (&t)[4]) {
+  if (p.teacher_type == kTypeF32) load4(static_cast<const float*>(p.teacher) + i, t);
+  else if (p.teacher_type == kTypeBf16) load4(static_cast<const __nv_bfloat16*>(p.teacher) + i, t);
+  else load4(static_cast<const __half*>(p.teacher) + i, t);
+}
 __device__ __forceinline__ float teacher_at(const DistillParams& p, int64_t i) {
   if (p.teacher_type == kTypeF32) return __ldg(static_cast<const float*>(p.teacher) + i);
   if (p.teacher_type == kTypeBf16) return to_f(static_cast<const __nv_bfloat16*>(p.teacher)[i]);
   return to_f(static_cast<const __half*>(p.teacher)[i]);
 }
-
-struct Entry {
-  float z;   // student's logit
-  float t;   // teacher's weight (not below 0) or logit
-  bool in;
-};
-// Entry j of row r; its column goes to *column.
+// The student's logit of an entry in column c (-inf: it takes no part).
 template <typename T>
-__device__ __forceinline__ Entry entry_at(const DistillParams& p, int64_t r, const T* row, int j, int* column) {
-  Entry e{0.f, 0.f, false};
-  const int c = p.indices ? __ldg(p.indices + r * p.K + j) : j;
-  *column = c;
-  if (c < 0 || c >= p.V) return e;
-  const float raw = to_f(row[c]);
-  e.in = !(raw == -INFINITY);
-  if (!e.in) return e;
-  const float t = teacher_at(p, r * p.K + j);
-  e.z = raw;
-  e.t = p.teacher_logits ? t : (t < 0.f ? 0.f : t);   // (NaN stays NaN)
-  return e;
+__device__ __forceinline__ float student_at(const DistillParams& p, const T* row, int c) {
+  return c >= 0 && c < p.V ? to_f(row[c]) : -INFINITY;
+}
+// Entries j0 .. j0 + 3 of row r: z the student's logit, -inf where the entry takes no part, t the teacher's (0 there).  p.quads: lists
+// come in aligned fours.
+template <typename T>
+__device__ __forceinline__ void entries4(const DistillParams& p, int64_t r, const T* row, int j0, float (&z)[4], float (&t)[4]) {
+  if (p.quads) {
+    if (p.indices) {
+      const int4 c = __ldg(reinterpret_cast<const int4*>(p.indices + r * p.K + j0));
+      z[0] = student_at(p, row, c.x); z[1] = student_at(p, row, c.y); z[2] = student_at(p, row, c.z); z[3] = student_at(p, row, c.w);
+    } else {
+      load4(row + j0, z);
+    }
+    teacher4(p, r * p.K + j0, t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i;
+      z[i] = -INFINITY;
+      t[i] = 0.f;
+      if (j < p.K) {
+        z[i] = student_at(p, row, p.indices ? __ldg(p.indices + r * p.K + j) : j);
+        t[i] = teacher_at(p, r * p.K + j);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (z[i] == -INFINITY) t[i] = p.teacher_logits ? -INFINITY : 0.f;   // (whatever the teacher holds there)
+    else if (!p.teacher_logits && t[i] < 0.f) t[i] = 0.f;
+  }
 }
 
-enum { kMax, kSum };
-// Reduction of two values over the block; every thread gets both.
-template <int kThreads, int kOp>
-__device__ __forceinline__ float2 block_reduce(float2 v, float2* scratch) {
-  auto op = [](float a, float b) { return kOp == kMax ? fmaxf(a, b) : a + b; };
+struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Sum { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+// Reduction over the block; every thread gets the result.  scratch: kThreads / 32 values of its own for every call.
+template <int kThreads, int kN, typename Op>
+__device__ __forceinline__ void block_reduce(float (&v)[kN], float (*scratch)[kN], Op op) {
+  constexpr int kWarps = kThreads / 32;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    v.x = op(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
-    v.y = op(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
   }
-  constexpr int kWarps = kThreads / 32;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) scratch[threadIdx.x >> 5][i] = v[i];
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x & (kWarps - 1)];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = scratch[threadIdx.x & (kWarps - 1)][i];
 #pragma unroll
   for (int o = kWarps / 2; o > 0; o >>= 1) {
-    v.x = op(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
-    v.y = op(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
   }
-  return v;
 }
 
-// Running maximum and sum of exponentials relative to it.
+// Running maximum m and sum s of exp((x - m) / T).
 struct Online {
   float m = kLowest, s = 0.f;
   template <int N>
@@ -112,68 +167,72 @@ struct Online {
   }
 };
 
-// The row's columns in 16-byte units from the first aligned one on; `one` takes a single column, `unit` a whole unit's first column.
-template <typename T, typename One, typename Unit>
-__device__ __forceinline__ void for_columns(const T* row, int n, int tid, int threads, One one, Unit unit) {
-  constexpr int kN = Vec<T>::kN;
-  int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T));
-  if (head > n) head = n;
-  const int units = (n - head) / kN, tail = head + units * kN;
-  if (tid < head) one(tid);
-  for (int u = tid; u < units; u += threads) unit(head + u * kN);
-  if (tail + tid < n) one(tail + tid);
-}
+// What a thread knows of its entries: zm, s as above over the entries; tm the teacher's largest logit (weights: unused), W = sum w,
+// A = sum w (log w - (z - zm) / T), with w = weight or exp((t - tm) / T).
+struct List {
+  Online z;
+  float tm = kLowest, W = 0.f, A = 0.f;
+  __device__ __forceinline__ void add(const DistillParams& p, const float (&zs)[4], const float (&ts)[4]) {
+    const float before = z.m;
+    z.add(zs, p.exp_scale);
+    if (z.m > before && W != 0.f) A += W * ((z.m - before) * p.inv_T);
+    if (p.teacher_logits) {
+      const float top = fmaxf(fmaxf(ts[0], ts[1]), fmaxf(ts[2], ts[3]));
+      if (top > tm) {
+        if (W != 0.f) {
+          const float f = exp_from(tm, top, p.exp_scale);
+          A = f > 0.f ? f * (A + W * ((tm - top) * p.inv_T)) : 0.f;
+          W *= f;
+        }
+        tm = top;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = p.teacher_logits ? exp_from(ts[i], tm, p.exp_scale) : ts[i];
+      if (w != 0.f) {   // (also keeps -inf out of a product with 0)
+        const float log_w = p.teacher_logits ? (ts[i] - tm) * p.inv_T : ln_of(w);
+        W += w;
+        A += w * (log_w + (z.m - zs[i]) * p.inv_T);
+      }
+    }
+  }
+};
 }  // namespace dt
 
 // -------------------------------------------------------------------------------------------------
-// forward: a block per row.  Each thread keeps kItems list entries in registers (0: they are read again for every pass).
+// forward: a block per row
 // -------------------------------------------------------------------------------------------------
-template <typename T, int kThreads, int kItems>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const __grid_constant__ DistillParams p) {
+template <typename T, int kThreads, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) distill_fwd_kernel(const __grid_constant__ DistillParams p) {
   using namespace dt;
-  __shared__ float2 scratch[32];
+  __shared__ float s_max[kThreads / 32][2], s_sum[kThreads / 32][3];
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const T* row = static_cast<const T*>(p.student) + r * p.row_stride;
 
-  Entry keep[kItems ? kItems : 1];
-  auto entries = [&](auto f) {
-    if constexpr (kItems) {
-#pragma unroll
-      for (int i = 0; i < kItems; ++i)
-        if (keep[i].in) f(keep[i]);
-    } else {
-      int c;
-      for (int j = tid; j < p.K; j += kThreads) {
-        const Entry e = entry_at<T>(p, r, row, j, &c);
-        if (e.in) f(e);
-      }
-    }
-  };
-  if constexpr (kItems) {
-    int c;
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int j = tid + i * kThreads;
-      keep[i] = j < p.K ? entry_at<T>(p, r, row, j, &c) : Entry{0.f, 0.f, false};
-    }
+  List list;
+  for (int j0 = tid * 4; j0 < p.K; j0 += kThreads * 4) {
+    float z[4], t[4];
+    entries4<T>(p, r, row, j0, z, t);
+    list.add(p, z, t);
   }
-  // maxima of the student's list (or, online, of the whole row) and of the teacher's logits
-  float2 top = make_float2(kLowest, kLowest), sum = make_float2(0.f, 0.f);
-  Online all;
+  Online all = list.z;
   if (p.over_row) {
-    constexpr int kN = Vec<T>::kN;
-    // four units in flight per thread
+    // the whole row, in 16-byte units from the first aligned one on, kUnroll of them on their way per thread
+    constexpr int kN = Vec<T>::kN, kUnroll = 2;
+    all = Online{};
     int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T));
     if (head > p.V) head = p.V;
     const int units = (p.V - head) / kN, tail = head + units * kN;
+    const T* body = row + head;
     int u = tid;
-    for (; u + 3 * kThreads < units; u += 4 * kThreads) {
-      Vec<T> v[4];
+    for (; u + (kUnroll - 1) * kThreads < units; u += kUnroll * kThreads) {
+      Vec<T> v[kUnroll];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i].load(row + head + (u + i * kThreads) * kN);
+      for (int i = 0; i < kUnroll; ++i) v[i].load(body + static_cast<int64_t>(u + i * kThreads) * kN);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kUnroll; ++i) {
         float z[kN];
 #pragma unroll
         for (int k = 0; k < kN; ++k) z[k] = v[i].get(k);
@@ -182,56 +241,49 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const __grid_cons
     }
     for (; u < units; u += kThreads) {
       Vec<T> v;
-      v.load(row + head + u * kN);
+      v.load(body + static_cast<int64_t>(u) * kN);
       float z[kN];
 #pragma unroll
       for (int k = 0; k < kN; ++k) z[k] = v.get(k);
       all.add(z, p.exp_scale);
     }
-    for (int side = 0; side < 2; ++side) {
-      const int c = side ? tail + tid : tid;
-      if (c < (side ? p.V : head)) {
-        float z[1] = {to_f(row[c])};
-        all.add(z, p.exp_scale);
-      }
-    }
-    top.x = all.m;
+    if (tid < head) { const float z[1] = {to_f(row[tid])}; all.add(z, p.exp_scale); }
+    if (tail + tid < p.V) { const float z[1] = {to_f(row[tail + tid])}; all.add(z, p.exp_scale); }
   }
-  entries([&](const Entry& e) {
-    if (!p.over_row) top.x = fmaxf(top.x, e.z);
-    if (p.teacher_logits) top.y = fmaxf(top.y, e.t);
-  });
-  top = block_reduce<kThreads, kMax>(top, scratch);
-  if (p.over_row) sum.x = all.s * exp_from(all.m, top.x, p.exp_scale);
-  entries([&](const Entry& e) {
-    if (!p.over_row) sum.x += exp_from(e.z, top.x, p.exp_scale);
-    sum.y += p.teacher_logits ? exp_from(e.t, top.y, p.exp_scale) : e.t;
-  });
-  sum = block_reduce<kThreads, kSum>(sum, scratch);
-  const bool active = !(sum.y == 0.f);   // (NaN: the loss says so)
-  const float log_s = logf(sum.x), log_w = logf(sum.y);
-  float2 loss = make_float2(0.f, 0.f);
-  if (active)
-    entries([&](const Entry& e) {
-      const float w = p.teacher_logits ? exp_from(e.t, top.y, p.exp_scale) : e.t;
-      if (!(w == 0.f)) loss.x += w / sum.y * ((p.teacher_logits ? (e.t - top.y) * p.inv_T : logf(w)) - log_w + (top.x - e.z) * p.inv_T + log_s);
-    });
-  loss = block_reduce<kThreads, kSum>(loss, scratch);
+  float top[2] = {all.m, list.tm};
+  block_reduce<kThreads>(top, s_max, Max());
+  // to the block's maxima
+  float sum[3] = {all.s * exp_from(all.m, top[0], p.exp_scale), list.W, list.A};
+  if (list.W != 0.f) {
+    sum[2] += list.W * ((top[0] - list.z.m) * p.inv_T);
+    if (p.teacher_logits) {
+      const float f = exp_from(list.tm, top[1], p.exp_scale);
+      sum[2] = f > 0.f ? f * (sum[2] + list.W * ((list.tm - top[1]) * p.inv_T)) : 0.f;
+      sum[1] *= f;
+    }
+  }
+  block_reduce<kThreads>(sum, s_sum, Sum());
   if (tid == 0) {
-    p.loss[r] = loss.x;
-    // for the backward: maximum and reciprocal sum of the student, maximum and sum of the teacher (sum 0: no gradient)
-    reinterpret_cast<float4*>(p.stats)[r] = make_float4(top.x, 1.f / sum.x, top.y, sum.y);
+    const float W = sum[1];
+    const bool active = !(W == 0.f);   // (NaN: the loss says so)
+    p.loss[r] = active ? sum[2] / W - logf(W) + logf(sum[0]) : 0.f;
+    // for the backward: maximum and reciprocal sum of the student; of the teacher the maximum of the logits, or a factor that keeps
+    // the weights' reciprocal sum finite, and that reciprocal (0: no gradient)
+    const float factor = p.teacher_logits ? 1.f : (W < 0x1p-100f ? 0x1p100f : 1.f);
+    reinterpret_cast<float4*>(p.stats)[r] =
+        make_float4(top[0], active ? 1.f / sum[0] : 0.f, p.teacher_logits ? top[1] : factor, active ? 1.f / (W * factor) : 0.f);
   }
 }
 
 namespace dt {
+// The teacher's probability of an entry that takes part.
 __device__ __forceinline__ float teacher_p(const DistillParams& p, const float4& st, float t) {
-  return (p.teacher_logits ? exp_from(t, st.z, p.exp_scale) : t) / st.w;
+  return (p.teacher_logits ? exp_from(t, st.z, p.exp_scale) : t * st.z) * st.w;
 }
 }  // namespace dt
 
 // -------------------------------------------------------------------------------------------------
-// backward without indices: element by element; block = (row, part of its columns)
+// backward without indices: four entries per thread and step; block = (row, part of its columns)
 // -------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) distill_bwd_kernel(const __grid_constant__ DistillParams p, const int parts) {
@@ -241,61 +293,87 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const __grid_constant_
   const T* row = static_cast<const T*>(p.student) + r * p.row_stride;
   T* out = static_cast<T*>(p.d_student) + r * p.V;
   const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
-  const float g = st.w == 0.f ? 0.f : __ldg(p.grad + r) * p.inv_T;
+  const bool active = !(st.w == 0.f);
+  const float g = active ? __ldg(p.grad + r) * p.inv_T : 0.f;
   const int n = min(p.V, (part + 1) * kChunk);
-#pragma unroll 4
-  for (int c = part * kChunk + static_cast<int>(threadIdx.x); c < n; c += 256) {
-    int column;
-    const Entry e = entry_at<T>(p, r, row, c, &column);
-    const float d = e.in && !(st.w == 0.f) ? g * (exp_from(e.z, st.x, p.exp_scale) * st.y - teacher_p(p, st, e.t)) : 0.f;
-    out[c] = from_f<T>(d);
+#pragma unroll 2
+  for (int c = part * kChunk + static_cast<int>(threadIdx.x) * 4; c < n; c += 256 * 4) {
+    float z[4], t[4], d[4];
+    entries4<T>(p, r, row, c, z, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      d[i] = active && !(z[i] == -INFINITY) ? g * (exp_from(z[i], st.x, p.exp_scale) * st.y - teacher_p(p, st, t[i])) : 0.f;
+    if (p.quads) store4(out + c, d);
+    else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < n) out[c + i] = static_cast<T>(d[i]);
+    }
   }
 }
 
 // -------------------------------------------------------------------------------------------------
-// backward with indices: block = (row, kChunk of its columns)
+// backward with indices: block = (row, kChunk of its columns).  kWide: rows in aligned 16-byte units, else element by element.
 // -------------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(512) distill_bwd_listed_kernel(const __grid_constant__ DistillParams p, const int parts) {
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(dt::kListedThreads) distill_bwd_listed_kernel(const __grid_constant__ DistillParams p, const int parts) {
   using namespace dt;
   __shared__ float acc[kChunk];
+  constexpr int kN = kWide ? Vec<T>::kN : 1, kUnits = kPerThread / kN;
   const int64_t r = blockIdx.x / parts;
   const int c0 = static_cast<int>(blockIdx.x - r * parts) * kChunk, n = min(p.V - c0, kChunk);
   const int tid = threadIdx.x;
   const T* row = static_cast<const T*>(p.student) + r * p.row_stride;
+  const T* src = row + c0;
   T* out = static_cast<T*>(p.d_student) + r * p.V + c0;
+  // the block's columns travel while the list is looked through
+  Vec<T> wide[kWide ? kUnits : 1];
+  float narrow[kWide ? 1 : kUnits];
+  if (p.over_row) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = (tid + u * kListedThreads) * kN;
+      if (c < n) {
+        if constexpr (kWide) wide[u].load(src + c);
+        else narrow[u] = to_f(src[c]);
+      }
+    }
+  }
   const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
   const bool active = !(st.w == 0.f);
   const float g = active ? __ldg(p.grad + r) * p.inv_T : 0.f;
-  for (int i = tid; i < n; i += 512) acc[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kChunk; i += kListedThreads * 4) *reinterpret_cast<float4*>(acc + i + tid * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  if (active)
-    for (int j = tid; j < p.K; j += 512) {
+  if (active) {
+#pragma unroll 4
+    for (int j = tid; j < p.K; j += kListedThreads) {
       const int c = __ldg(p.indices + r * p.K + j) - c0;
       if (c < 0 || c >= n) continue;
-      int column;
-      const Entry e = entry_at<T>(p, r, row, j, &column);
-      if (!e.in) continue;
-      const float soft = p.over_row ? 0.f : exp_from(e.z, st.x, p.exp_scale) * st.y;
-      atomicAdd(&acc[c], g * (soft - teacher_p(p, st, e.t)));
+      const float z = to_f(src[c]);
+      if (z == -INFINITY) continue;
+      float t = teacher_at(p, r * p.K + j);
+      if (!p.teacher_logits && t < 0.f) t = 0.f;
+      const float soft = p.over_row ? 0.f : exp_from(z, st.x, p.exp_scale) * st.y;
+      atomicAdd(&acc[c], g * (soft - teacher_p(p, st, t)));
     }
+  }
   __syncthreads();
-  const T* src = row + c0;
-  const float scale = p.over_row ? g * st.y : 0.f;
-  auto value = [&](float raw, int c) {
-    return p.over_row && active ? fmaf(scale, exp_from(raw, st.x, p.exp_scale), acc[c]) : acc[c];
-  };
-  if (((reinterpret_cast<uintptr_t>(src) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
-    for_columns(src, n, tid, 512, [&](int c) { out[c] = from_f<T>(value(p.over_row ? to_f(src[c]) : 0.f, c)); },
-                [&](int c) {
-                  Vec<T> v, o;
-                  if (p.over_row) v.load(src + c);
+  const float scale = g * st.y;
+  auto value = [&](float z, int c) { return p.over_row && active ? fmaf(scale, exp_from(z, st.x, p.exp_scale), acc[c]) : acc[c]; };
 #pragma unroll
-                  for (int k = 0; k < Vec<T>::kN; ++k) o.set(k, value(p.over_row ? v.get(k) : 0.f, c + k));
-                  o.store(out + c);
-                });
-  } else {
-    for (int c = tid; c < n; c += 512) out[c] = from_f<T>(value(p.over_row ? to_f(src[c]) : 0.f, c));
+  for (int u = 0; u < kUnits; ++u) {
+    const int c = (tid + u * kListedThreads) * kN;
+    if (c < n) {
+      if constexpr (kWide) {
+        Vec<T> o;
+#pragma unroll
+        for (int k = 0; k < kN; ++k) o.set(k, value(wide[u].get(k), c + k));
+        o.store(out + c);
+      } else {
+        out[c] = static_cast<T>(value(narrow[u], c));
+      }
+    }
   }
 }
 
@@ -303,17 +381,17 @@ __global__ void __launch_bounds__(512) distill_bwd_listed_kernel(const __grid_co
 // host side
 // -------------------------------------------------------------------------------------------------
 namespace {
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+size_t type_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
+
 template <typename T>
-int forward(const DistillParams& p, cudaStream_t stream) {
+int forward(const DistillParams& p, int sms, cudaStream_t stream) {
   const unsigned rows = static_cast<unsigned>(p.rows);
-  // a whole row of many columns is worth more threads; a list stays in registers where it fits
-  if (p.over_row && p.V > 4096) {
-    if (p.K <= 2048) distill_fwd_kernel<T, 512, 4><<<rows, 512, 0, stream>>>(p);
-    else if (p.K <= 8192) distill_fwd_kernel<T, 512, 16><<<rows, 512, 0, stream>>>(p);
-    else distill_fwd_kernel<T, 512, 0><<<rows, 512, 0, stream>>>(p);
-  } else if (p.K <= 1024) distill_fwd_kernel<T, 256, 4><<<rows, 256, 0, stream>>>(p);
-  else if (p.K <= 4096) distill_fwd_kernel<T, 256, 16><<<rows, 256, 0, stream>>>(p);
-  else distill_fwd_kernel<T, 256, 0><<<rows, 256, 0, stream>>>(p);
+  // Whole rows: many of them run side by side in blocks of 256 threads, eight to an SM (1024 rows in blocks of 512 are 1.7 rounds of
+  // the chip); few rows take 1024 threads each.  Lists: 256 threads, 64 where that is four entries each.
+  if (p.over_row && p.V > 4096 && p.rows < 2 * sms) distill_fwd_kernel<T, 1024, 1><<<rows, 1024, 0, stream>>>(p);
+  else if (!p.over_row && p.K <= 256) distill_fwd_kernel<T, 64, 1><<<rows, 64, 0, stream>>>(p);
+  else distill_fwd_kernel<T, 256, 8><<<rows, 256, 0, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T>
@@ -321,19 +399,35 @@ int backward(const DistillParams& p, cudaStream_t stream) {
   const int parts = (p.V + dt::kChunk - 1) / dt::kChunk;
   const int64_t blocks = p.rows * parts;
   if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  if (p.indices) distill_bwd_listed_kernel<T><<<static_cast<unsigned>(blocks), 512, 0, stream>>>(p, parts);
-  else distill_bwd_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, parts);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  const int n = dt::Vec<T>::kN;
+  if (!p.indices) distill_bwd_kernel<T><<<grid, 256, 0, stream>>>(p, parts);
+  else if (p.V % n == 0 && p.row_stride % n == 0 && aligned(p.student, 16) && aligned(p.d_student, 16))
+    distill_bwd_listed_kernel<T, true><<<grid, dt::kListedThreads, 0, stream>>>(p, parts);
+  else
+    distill_bwd_listed_kernel<T, false><<<grid, dt::kListedThreads, 0, stream>>>(p, parts);
   return static_cast<int>(cudaGetLastError());
+}
+void finish(DistillParams* p) {
+  if (!p->indices) p->over_row = 0;   // the list is the row
+  // fours of a list: the indices, or without them the student's row (and its gradient), and the teacher's entries
+  const size_t own = type_bytes(p->student_type);
+  p->quads = p->K % 4 == 0 && aligned(p->teacher, 4 * type_bytes(p->teacher_type)) &&
+             (p->indices ? aligned(p->indices, 16)
+                         : p->row_stride % 4 == 0 && aligned(p->student, 4 * own) && (!p->d_student || aligned(p->d_student, 4 * own)));
 }
 }  // namespace
 
 int launch_distill_fwd(DistillParams p, cudaStream_t stream) {
-  if (!p.indices) p.over_row = 0;   // the list is the row
-  if (p.student_type == kTypeF32) return forward<float>(p, stream);
-  return p.student_type == kTypeBf16 ? forward<__nv_bfloat16>(p, stream) : forward<__half>(p, stream);
+  int dev = 0, sms = 0;
+  cudaError_t e = current_device_sms(&dev, &sms);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  finish(&p);
+  if (p.student_type == kTypeF32) return forward<float>(p, sms, stream);
+  return p.student_type == kTypeBf16 ? forward<__nv_bfloat16>(p, sms, stream) : forward<__half>(p, sms, stream);
 }
 int launch_distill_bwd(DistillParams p, cudaStream_t stream) {
-  if (!p.indices) p.over_row = 0;
+  finish(&p);
   if (p.student_type == kTypeF32) return backward<float>(p, stream);
   return p.student_type == kTypeBf16 ? backward<__nv_bfloat16>(p, stream) : backward<__half>(p, stream);
 }

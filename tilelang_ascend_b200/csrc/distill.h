@@ -18,6 +18,7 @@ struct DistillParams {
   int64_t rows, row_stride;
   int V, K;
   int student_type, teacher_type, teacher_logits, over_row;
+  int quads;                // set by the launcher: lists in aligned fours
   float inv_T, exp_scale;   // 1 / T, log2(e) / T
 };
 

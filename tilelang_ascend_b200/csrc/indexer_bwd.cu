@@ -49,14 +49,14 @@ __global__ void __launch_bounds__(ib::kThreads, 2) indexer_bwd_kernel(const __gr
     return;
   }
   const uint32_t sK = sQ + kOffK, sDz = sQ + kOffDz;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + kOffBar);   // [2] count 128: the gather threads' copies have landed
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + kOffBar);   // [2] count 4: the gather warps' copies have landed
   uint64_t* k_empty = k_full + 2;    // [2] count 1: commit after the MMAs that read the stage
   uint64_t* z_full = k_full + 4;     // count 1: commit after Z
-  uint64_t* z_free = k_full + 5;     // count 256: the workers have read Z
-  uint64_t* dz_full = k_full + 6;    // count 256: dZ is in shared memory
+  uint64_t* z_free = k_full + 5;     // count 8: the workers have read Z
+  uint64_t* dz_full = k_full + 6;    // count 8: dZ is in shared memory
   uint64_t* dz_free = k_full + 7;    // count 1: commit after the MMAs that read dZ
   uint64_t* dk_full = k_full + 8;    // count 1: commit after dK^T
-  uint64_t* dk_free = k_full + 9;    // count 256: the workers have read dK^T
+  uint64_t* dk_free = k_full + 9;    // count 8: the workers have read dK^T
   uint64_t* q_full = k_full + 10;    // count 256: the query's heads have landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_full + 11);
   int* start_status = reinterpret_cast<int*>(k_full + 12);
@@ -73,9 +73,9 @@ __global__ void __launch_bounds__(ib::kThreads, 2) indexer_bwd_kernel(const __gr
 
   if (tid == 0) {
     *start_status = *reinterpret_cast<volatile int*>(p.status);
-    for (int i = 0; i < kStages; ++i) { mbar_init(&k_full[i], 128); mbar_init(&k_empty[i], 1); }
-    mbar_init(z_full, 1); mbar_init(z_free, kWorkers * 32); mbar_init(dz_full, kWorkers * 32); mbar_init(dz_free, 1);
-    mbar_init(dk_full, 1); mbar_init(dk_free, kWorkers * 32); mbar_init(q_full, kWorkers * 32);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); }
+    mbar_init(z_full, 1); mbar_init(z_free, kWorkers); mbar_init(dz_full, kWorkers); mbar_init(dz_free, 1);
+    mbar_init(dk_full, 1); mbar_init(dk_free, kWorkers); mbar_init(q_full, kWorkers * 32);
     mbar_init_fence();
   }
   if (tid < kHeads) s_w[tid] = tid < p.N1 ? p.w[static_cast<int64_t>(bt) * p.N1 + tid] : 0.f;
@@ -139,9 +139,12 @@ __global__ void __launch_bounds__(ib::kThreads, 2) indexer_bwd_kernel(const __gr
         cp_async16(dst + sw128_offset(key0 + 4 * i, unit), src, idx[i] < 0 ? 0u : 16u);
         cp_async16(dst + kKChunk + sw128_offset(key0 + 4 * i, unit), src + 64, idx[i] < 0 ? 0u : 16u);
       }
-      cp_async_arrive_noinc(&k_full[s]);
+      cp_async_commit();
+      // a warp announces a tile once, when its copies have landed (128 threads arriving by themselves hold the barrier up)
+      cp_async_wait<0>();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[s]);
     }
-    cp_async_wait<0>();
   } else if (warp == kMmaWarp) {
     // ================================ MMA issuer (converged, one elected lane issues) ===============
     constexpr uint32_t id_z = make_idesc_f16(kBF16, kKeys, kHeads, 0, 0);
@@ -227,7 +230,8 @@ __global__ void __launch_bounds__(ib::kThreads, 2) indexer_bwd_kernel(const __gr
         }
       }
       tc_fence_before();
-      mbar_arrive(dk_free);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dk_free);
       return true;
     };
     // dZ of tile number g, and its part of dw
@@ -266,9 +270,12 @@ __global__ void __launch_bounds__(ib::kThreads, 2) indexer_bwd_kernel(const __gr
         st_shared_v4(sDz + sw128_offset(key, unit + 1), w[4], w[5], w[6], w[7]);
       }
       tc_fence_before();
-      mbar_arrive(z_free);
       fence_proxy_async_smem();
-      mbar_arrive(dz_full);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(z_free);
+        mbar_arrive(dz_full);
+      }
       return true;
     };
     int g = 0;

@@ -365,19 +365,21 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
   for (int i = tid; i < p.norm_dim; i += kThreads) { line[i] = sdw[i]; line[p.norm_dim + i] = sdb[i]; }
 }
 
-// dweight and dbias from the blocks' lines: a block takes 32 columns of the 2 * norm_dim, its warps every eighth line.
+// dweight and dbias from the blocks' lines: a block takes 32 columns of the 2 * norm_dim, its warps every 32nd line (every eighth, of twice
+// as many lines: 8.8 us for 128 dims).
 template <typename T>
-__global__ void __launch_bounds__(256) norm_rope_param_grad_kernel(const float* partials, int lines, int norm_dim, void* d_weight, void* d_bias, int fp32) {
-  __shared__ float sums[8][33];
+__global__ void __launch_bounds__(1024) norm_rope_param_grad_kernel(const float* partials, int lines, int norm_dim, void* d_weight, void* d_bias, int fp32) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < 2 * norm_dim)
-    for (int l = warp; l < lines; l += 8) s += partials[static_cast<long long>(l) * 2 * norm_dim + c];
+#pragma unroll 4
+    for (int l = warp; l < lines; l += 32) s += partials[static_cast<long long>(l) * 2 * norm_dim + c];
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < 2 * norm_dim) {
     s = 0.f;
-    for (int w = 0; w < 8; ++w) s += sums[w][lane];
+    for (int w = 0; w < 32; ++w) s += sums[w][lane];
     void* out = c < norm_dim ? d_weight : d_bias;
     const int i = c < norm_dim ? c : c - norm_dim;
     if (out) {
@@ -532,12 +534,12 @@ void tile(NormRopeParams* p, int which, int rows) {
   sd.tile_tokens = tokens < 1 ? 1 : tokens;
   sd.blocks = ((p->tokens + sd.tile_tokens - 1) / sd.tile_tokens) * ((sd.H + sd.tile_heads - 1) / sd.tile_heads);
 }
-// Rows per block: 64 amortise a block's angles and weights; calls that would not fill the SMs twice take shorter blocks.
+// Rows per block: 64 amortise a block's angles and weights; calls of fewer than four blocks per SM take shorter ones.
 void tiles(NormRopeParams* p, int sms) {
   for (int rows = 64; rows >= 8; rows >>= 1) {
     tile(p, 0, rows);
     tile(p, 1, rows);
-    if (p->side[0].blocks + p->side[1].blocks >= 2 * sms) return;
+    if (p->side[0].blocks + p->side[1].blocks >= 4 * sms) return;
   }
 }
 int tile_smem(const NormRopeParams& p) {
@@ -581,7 +583,7 @@ int backward_units(const NormRopeParams& p, int grid, cudaStream_t stream) {
   return backward<T, 32, 4>(p, grid, stream);
 }
 // Blocks of a backward with a norm: every block leaves one line of sums.
-int norm_lines(int sms) { return 4 * sms; }
+int norm_lines(int sms) { return 2 * sms; }
 }  // namespace
 
 int launch_norm_rope(NormRopeParams p, bool bf16, cudaStream_t stream) {
@@ -642,9 +644,9 @@ int launch_norm_rope_bwd(NormRopeParams p, void* const d_weight[2], void* const 
     if (!one.side[0].partials) continue;
     const int cols = (2 * p.norm_dim + 31) / 32;
     if (bf16)
-      norm_rope_param_grad_kernel<__nv_bfloat16><<<cols, 256, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
+      norm_rope_param_grad_kernel<__nv_bfloat16><<<cols, 1024, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
     else
-      norm_rope_param_grad_kernel<__half><<<cols, 256, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
+      norm_rope_param_grad_kernel<__half><<<cols, 1024, 0, stream>>>(one.side[0].partials, grid, p.norm_dim, d_weight[i], d_bias[i], one.side[0].param_fp32);
     if ((err = static_cast<int>(cudaGetLastError()))) return err;
   }
   return 0;

@@ -4,11 +4,16 @@
 //
 // what the sparse MLA forward's softmax gives each key of a query's list; the forward keeps only its normaliser (lse).
 //
-// Bound by the tensor cores on paper (2 H D operations against 2 D gathered bytes per key).  The MMA is issued transposed:
-// A = 128 gathered keys x 64 dims at a time (UMMA M = keys), B = up to 128 heads of the query, so that the accumulator holds a
-// key per lane and the sum over heads is each thread's own, without exchange; 128 exponentials per key cost half of its MMA time.
-// The query's heads stay in shared memory, the keys pass through a ring of chunks of [128 keys x 64 dims].  One CTA per query,
-// long (late) queries first; more than 128 heads take further passes over the list.
+// Bound by the tensor cores on paper (2 H D operations against 2 D gathered bytes per key), by shared memory in practice: a
+// tile of 128 keys x 576 dims is written once (1152 clocks of the SM's 128 B/clk) and read once by the MMAs that take 2304 clocks.
+// So the other operand must not come from there: S = Q K^T with A = the query's 128 heads, eight of their 64-dim chunks in tensor
+// memory (256 columns, beside two score accumulators of 128), the rest in shared memory, B = the gathered keys.  (With the
+// heads in shared memory too -- transposed product, a key per lane and no exchange in the sum over heads -- a tile's operands
+// take 3456 clocks of shared memory and leave room for five stages of the ring: 1093 us for 4096 queries of 2048 keys x 128 heads.)
+// Persistent CTAs, one per SM, long (late) queries first.  A query's heads ride the ring ahead of its keys and are moved to
+// tensor memory by the epilogue warps as soon as the last MMAs of the query before are done, so that the gather never stops.
+// Warps: 8 epilogue (quarter of the heads x half of the keys), 8 gather, the MMA issuer, and one that reads the next query's list.
+// The sum over heads goes over the lanes by halving exchanges (31 shuffles for 32 keys), then over the four quarters.
 #include <type_traits>
 
 #include "fwd_common.cuh"
@@ -17,17 +22,53 @@
 namespace dsa {
 
 namespace kw {
-constexpr int kKeys = 128;                        // keys per tile = UMMA M
-constexpr int kHeads = 128;                       // heads per pass, at most (UMMA N = the next multiple of 16)
-constexpr uint32_t kChunkBytes = kKeys * 128;     // 128 keys x 64 dims
-constexpr int kMaxStages = 12;
+// Barrier over nthreads threads that tells all of them whether all of them say yes.
+__device__ __forceinline__ bool bar_and(uint32_t id, uint32_t nthreads, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(yes ? 1u : 0u), "r"(id), "r"(nthreads)
+      : "memory");
+  return all != 0;
+}
+
+constexpr int kKeys = 128;                        // keys per tile = UMMA N
+constexpr int kHeads = 128;                       // heads per pass over the list = UMMA M
+constexpr uint32_t kChunkBytes = 128 * 128;       // 128 keys (or heads) x 64 dims
+constexpr int kTmemChunks = 8;                    // chunks of the heads in tensor memory
+constexpr int kPerStage = 3;                       // chunks of a stage of the ring
+constexpr uint32_t kStageBytes = kPerStage * kChunkBytes;
+constexpr int kMaxStages = 4;
 constexpr int kMaxWords = 8192 / 32;              // validity bits of a list
-constexpr int kGatherWarps = 8, kMmaWarp = 12, kThreads = 13 * 32;   // warps 0-3: query rows, then epilogue
-constexpr uint32_t kFixedBytes = 256 + kHeads * 4 + kMaxWords * 4;   // barriers, lse, bits
+constexpr int kEpilogueWarps = 8, kGatherWarps = 8, kMmaWarp = 16, kListWarp = 17, kThreads = 18 * 32;
+constexpr int kUsers = kEpilogueWarps + kGatherWarps + 1;   // warps that read a list
+constexpr uint32_t kOffBits = 512;                              // after the barriers: two lists
+constexpr uint32_t kListBytes = kMaxWords * 4 + 16 + kMaxWords / 4;   // validity bits; number of tiles with a key; those tiles
+constexpr uint32_t kOffPart = kOffBits + 2 * kListBytes;        // two tiles' sums of the four quarters
+constexpr uint32_t kFixedBytes = kOffPart + 2 * 4 * kKeys * 4;
 constexpr uint32_t kMaxSmem = 232448;
-constexpr uint32_t kTmemCols = 2 * kHeads;        // two accumulators
+constexpr uint32_t kColS = kTmemChunks * 32, kTmemCols = 512;
+static_assert(kColS + 2 * kKeys <= kTmemCols, "tensor memory columns");
 struct Shape {
-  int chunks, n, stages;                          // 64-dim chunks of a row; UMMA N; stages of the ring
+  int chunks, parts;         // 64-dim chunks of a row; stages that a row tile passes through
+  int smem_chunks, stages;   // chunks of the heads in shared memory; stages of the ring
+};
+
+// Position in the ring.
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) { stage = 0; phase ^= 1u; }
+  }
+  __device__ __forceinline__ void skip(int n, int stages) {
+    stage += n;
+    while (stage >= stages) { stage -= stages; phase ^= 1u; }
+  }
 };
 }  // namespace kw
 
@@ -42,167 +83,341 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
     if (threadIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusBadLayout);
     return;
   }
-  const uint32_t q_chunk = static_cast<uint32_t>(sh.n) * 128;      // one chunk of the query's heads
-  const uint32_t sK = sQ + sh.chunks * q_chunk;
-  uint8_t* fixed = smem + sh.chunks * q_chunk + sh.stages * kChunkBytes;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(fixed);   // [kMaxStages] count 256: the gather threads' copies have landed
-  uint64_t* k_empty = k_full + kMaxStages;                 // [kMaxStages] count 1: commit after the MMAs that read the stage
+  const uint32_t sK = sQ + sh.smem_chunks * kChunkBytes;
+  uint8_t* fixed = smem + sh.smem_chunks * kChunkBytes + sh.stages * kStageBytes;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(fixed);   // [kMaxStages] count 128: a gather group's copies have landed
+  uint64_t* k_empty = k_full + kMaxStages;                 // [kMaxStages] count 1: commit after the MMAs that read the stage, or the heads have been moved on
   uint64_t* acc_full = k_empty + kMaxStages;               // [2] count 1: commit after a tile's last MMA
-  uint64_t* acc_empty = acc_full + 2;                      // [2] count 128
-  uint64_t* q_full = acc_empty + 2;                        // count 128: this pass's heads have landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+  uint64_t* acc_free = acc_full + 2;                       // [2] count 8: the epilogue warps have read the scores
+  uint64_t* q_ready = acc_free + 2;                        // count 8: a pass's heads are in place
+  uint64_t* list_full = q_ready + 1;                       // [2] count 1
+  uint64_t* list_free = list_full + 2;                     // [2] count kUsers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(list_free + 2);
   int* start_status = reinterpret_cast<int*>(tmem_slot + 1);
-  float* s_lse = reinterpret_cast<float*>(fixed + 256);    // in log2 units; +inf: no weight
-  uint32_t* s_bits = reinterpret_cast<uint32_t*>(fixed + 256 + kHeads * 4);
+  float* s_part = reinterpret_cast<float*>(fixed + kOffPart);
+  auto bits_of = [&](int item) { return reinterpret_cast<uint32_t*>(fixed + kOffBits + (item & 1) * kListBytes); };
+  auto tiles_of = [&](int item) { return fixed + kOffBits + (item & 1) * kListBytes + kMaxWords * 4 + 16; };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int bt = p.B * p.S - 1 - static_cast<int>(blockIdx.x);
-  const RowCtx c = make_row_ctx(p, bt);
-  const int words = (p.topk + 31) >> 5, tiles = (p.topk + kKeys - 1) / kKeys;
-  float* out = weights + static_cast<int64_t>(bt) * p.topk;
+  const int n = p.B * p.S, tiles = (p.topk + kKeys - 1) / kKeys;
+  const int passes = (p.H + kHeads - 1) / kHeads;
+  // items of this CTA: queries n - 1 - blockIdx.x, then every gridDim.x-th before it
+  const int items = (n - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  auto query_of = [&](int item) { return n - 1 - static_cast<int>(blockIdx.x) - item * static_cast<int>(gridDim.x); };
 
   if (tid == 0) {
     *start_status = *reinterpret_cast<volatile int*>(p.status);
-    for (int i = 0; i < sh.stages; ++i) { mbar_init(&k_full[i], kGatherWarps * 32); mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 128); }
-    mbar_init(q_full, 128);
+    for (int i = 0; i < sh.stages; ++i) { mbar_init(&k_full[i], kGatherWarps * 16); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1); mbar_init(&acc_free[i], kEpilogueWarps);
+      mbar_init(&list_full[i], 1); mbar_init(&list_free[i], kUsers);
+    }
+    mbar_init(q_ready, kEpilogueWarps);
     mbar_init_fence();
-  }
-  for (int w = warp; w < 4 * tiles; w += kThreads / 32) {
-    const int j = w * 32 + lane;
-    const bool valid = w < words && j < p.topk && c.active && index_valid(c, __ldg(c.idx_row + j));
-    const uint32_t bits = __ballot_sync(0xffffffffu, valid);
-    if (lane == 0) s_bits[w] = bits;
   }
   if (warp == kMmaWarp) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const bool run = *start_status == kStatusOk;
-  const int passes = (p.H + kHeads - 1) / kHeads;
-  auto any_key = [&](int tile) { return (s_bits[4 * tile] | s_bits[4 * tile + 1] | s_bits[4 * tile + 2] | s_bits[4 * tile + 3]) != 0u; };
-
-  if (warp >= 4 && warp < kMmaWarp) {
-    // ================================ gather: 16 keys of every chunk per warp =======================
-    const int key0 = (warp - 4) * 16 + (lane >> 3), unit = lane & 7;   // this thread's keys: key0 + 4 i, one 16-byte unit of each
-    const T* kv = reinterpret_cast<const T*>(p.kv) + static_cast<int64_t>(c.b) * p.S_kv * p.D;
-    int stage = 0;
-    uint32_t phase = 1;   // (the first round of the ring finds its stages empty)
-    bool ok = run;
-    for (int pass = 0; ok && pass < passes; ++pass)
-      for (int tile = 0; ok && tile < tiles; ++tile) {
-        if (!any_key(tile)) continue;
-        const T* src[4];
-        uint32_t there = 0;
+  bool ok = *start_status == kStatusOk;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
+  if (warp == kListWarp) {
+    // ================================ lists: validity bits, one query ahead =========================
+    for (int item = 0; ok && item < items; ++item) {
+      if (item >= 2 && !wait(&list_free[item & 1], ((item >> 1) + 1) & 1)) { ok = false; break; }
+      const RowCtx c = make_row_ctx(p, query_of(item));
+      uint32_t* bits = bits_of(item);
+      uint8_t* list = tiles_of(item);
+      uint32_t count = 0;
+      for (int t0 = 0; t0 < tiles; t0 += 4) {   // four tiles' indices on their way at once
+        int idx[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 4 * i, slot = tile * kKeys + key;
-          const bool valid = (s_bits[slot >> 5] >> (slot & 31)) & 1u;
-          const int idx = valid ? __ldg(c.idx_row + slot) : 0;
-          src[i] = kv + static_cast<int64_t>(idx) * p.D + unit * 8;
-          there |= valid ? 1u << i : 0u;
+        for (int i = 0; i < 16; ++i) {
+          const int j = t0 * kKeys + i * 32 + lane;
+          idx[i] = j < p.topk ? __ldg(c.idx_row + j) : -1;
         }
-        for (int ch = 0; ch < sh.chunks; ++ch) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[stage], phase, p.status))) { ok = false; break; }
-          const bool dims = ch * 64 + unit * 8 < p.D;
-          const uint32_t dst = sK + stage * kChunkBytes;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool copy = dims && ((there >> i) & 1u);
-            cp_async16(dst + sw128_offset(key0 + 4 * i, unit), copy ? src[i] + ch * 64 : reinterpret_cast<const T*>(p.kv), copy ? 16u : 0u);
+        for (int t = 0; t < 4; ++t) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 4 * t; i < 4 * t + 4; ++i) {
+            const uint32_t b = __ballot_sync(0xffffffffu, c.active && index_valid(c, idx[i]));
+            if (lane == 0 && t0 + t < tiles) bits[t0 * 4 + i] = b;
+            any |= b;
           }
-          cp_async_arrive_noinc(&k_full[stage]);
-          if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
+          if (any) {
+            if (lane == 0) list[count] = static_cast<uint8_t>(t0 + t);
+            ++count;
+          }
         }
       }
+      if (lane == 0) {
+        bits[kMaxWords] = count;
+        mbar_arrive(&list_full[item & 1]);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= kEpilogueWarps && warp < kMmaWarp) {
+    // ================================ gather: 32 rows of every other stage per warp =================
+    // Two groups of four warps take alternate stages: waiting for a stage, announcing it and the loop around cost a warp as much as
+    // twelve copies.
+    const int group = (warp - kEpilogueWarps) >> 2, row0 = ((warp - kEpilogueWarps) & 3) * 32 + (lane >> 3), unit = lane & 7;   // rows row0 + 4 i
+    const T* none = reinterpret_cast<const T*>(p.kv);
+    Ring ring;
+    ring.phase = 1;   // (the first round of the ring finds its stages empty)
+    ring.skip(group, sh.stages);
+    int turn = group;   // stages until this group's next one
+    // eight rows per thread, stage by stage (base: this thread's unit of row 0's first chunk; row -1: zeros)
+    auto load_rows = [&](const T* base, const int (&row)[8]) {
+      for (; turn < sh.parts; turn += 2) {
+        if (!wait(&k_empty[ring.stage], ring.phase)) return false;
+#pragma unroll
+        for (int c = 0; c < kPerStage; ++c) {
+          const int ch = turn * kPerStage + c;
+          if (ch < sh.chunks) {
+            const bool dims = ch * 64 + unit * 8 < p.D;
+            const uint32_t dst = sK + ring.stage * kStageBytes + c * kChunkBytes;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bool copy = dims && row[i] >= 0;
+              cp_async16(dst + sw128_offset(row0 + 4 * i, unit), copy ? base + static_cast<int64_t>(row[i]) * p.D + ch * 64 : none, copy ? 16u : 0u);
+            }
+          }
+        }
+        cp_async_arrive_noinc(&k_full[ring.stage]);
+        ring.skip(2, sh.stages);
+      }
+      turn -= sh.parts;
+      return true;
+    };
+    for (int item = 0; ok && item < items; ++item) {
+      if (!wait(&list_full[item & 1], (item >> 1) & 1)) { ok = false; break; }
+      const uint32_t* bits = bits_of(item);
+      const uint8_t* list = tiles_of(item);
+      const int count = bits[kMaxWords];
+      if (count) {
+        const int bt = query_of(item);
+        const RowCtx c = make_row_ctx(p, bt);
+        const T* kv = reinterpret_cast<const T*>(p.kv) + static_cast<int64_t>(c.b) * p.S_kv * p.D + unit * 8;
+        const T* q = reinterpret_cast<const T*>(p.q) + static_cast<int64_t>(bt) * p.H * p.D + unit * 8;
+        auto indices = [&](int i, int (&row)[8]) {   // of the list's tile number i
+          const int slot0 = list[i] * kKeys + row0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int slot = slot0 + 4 * k;
+            row[k] = (bits[slot >> 5] >> (slot & 31)) & 1u ? __ldg(c.idx_row + slot) : -1;
+          }
+        };
+        for (int pass = 0; ok && pass < passes; ++pass) {
+          int row[8], next[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int h = pass * kHeads + row0 + 4 * i;
+            row[i] = h < p.H ? h : -1;
+          }
+          indices(0, next);
+          ok = load_rows(q, row);
+          for (int i = 0; ok && i < count; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) row[k] = next[k];
+            if (i + 1 < count) indices(i + 1, next);   // one tile ahead of its copies
+            ok = load_rows(kv, row);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_free[item & 1]);
+    }
     cp_async_wait<0>();
   } else if (warp == kMmaWarp) {
     // ================================ MMA issuer (converged, one elected lane issues) ===============
-    const uint32_t idesc = make_idesc_f16(kBF16, kKeys, sh.n, 0, 0), go = elect_one_lane();
-    int stage = 0, g = 0;
-    uint32_t phase = 0;
-    bool ok = run;
-    for (int pass = 0; ok && pass < passes; ++pass) {
-      bool first = true;
-      for (int tile = 0; ok && tile < tiles; ++tile) {
-        if (!any_key(tile)) continue;
-        if (first) {
-          if (!__all_sync(0xffffffffu, mbar_wait(q_full, pass & 1, p.status))) { ok = false; break; }
-          first = false;
-        }
-        const int a = g & 1;
-        if (g >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[a], ((g >> 1) + 1) & 1, p.status))) { ok = false; break; }
-        for (int ch = 0; ch < sh.chunks; ++ch) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&k_full[stage], phase, p.status))) { ok = false; break; }
-          fence_proxy_async_smem();   // the rows were written by cp.async of other threads
-          tc_fence_after();
-          const uint64_t da = make_smem_desc(sK + stage * kChunkBytes, 16, 1024, kSwizzle128B);
-          const uint64_t db = make_smem_desc(sQ + ch * q_chunk, 16, 1024, kSwizzle128B);
+    constexpr uint32_t idesc = make_idesc_f16(kBF16, kHeads, kKeys, 0, 0);
+    const uint32_t go = elect_one_lane();
+    Ring ring;
+    int g = 0, loads = 0;   // tiles and passes so far
+    // A barrier is looked at ahead of the work before it (the answer takes 200 clocks on this busy shared memory); `yes`: it was complete.
+    auto ready = [&](bool yes, uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, yes) || wait(bar, parity); };
+    for (int item = 0; ok && item < items; ++item) {
+      if (!wait(&list_full[item & 1], (item >> 1) & 1)) { ok = false; break; }
+      const int count = bits_of(item)[kMaxWords];
+      for (int pass = 0; ok && count && pass < passes; ++pass) {
+        ring.skip(sh.parts, sh.stages);   // the heads' slots are the epilogue warps'
+        if (!wait(q_ready, loads & 1)) { ok = false; break; }
+        ++loads;
+        bool full = mbar_try_wait(&k_full[ring.stage], ring.phase), room = g < 2 || mbar_try_wait(&acc_free[g & 1], ((g >> 1) + 1) & 1);
+        for (int i = 0; ok && i < count; ++i) {
+          const int a = g & 1;
+          if (g >= 2 && !ready(room, &acc_free[a], ((g >> 1) + 1) & 1)) { ok = false; break; }
+          const uint32_t acc = tmem_base + kColS + a * kKeys;
+          for (int part = 0; part < sh.parts; ++part) {
+            if (!ready(full, &k_full[ring.stage], ring.phase)) { ok = false; break; }
+            Ring after = ring;
+            after.next(sh.stages);
+            full = mbar_try_wait(&k_full[after.stage], after.phase);
+            fence_proxy_async_smem();   // the rows were written by cp.async of other threads
+            tc_fence_after();
+            const uint64_t db = make_smem_desc(sK + ring.stage * kStageBytes, 16, 1024, kSwizzle128B);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_ss_if(go, tmem_base + a * kHeads, da + 2 * k, db + 2 * k, idesc, (ch | k) != 0);
-          umma_commit_if(go, &k_empty[stage]);
-          if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
+            for (int c = 0; c < kPerStage; ++c) {
+              const int ch = part * kPerStage + c;
+              if (ch < kTmemChunks && ch < sh.chunks) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_ts_if(go, acc, tmem_base + (ch * 4 + k) * 8, db + ((c * kChunkBytes + k * 32) >> 4), idesc, (ch | k) != 0);
+              } else if (ch < sh.chunks) {
+                const uint64_t da = make_smem_desc(sQ + (ch - kTmemChunks) * kChunkBytes, 16, 1024, kSwizzle128B);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_ss_if(go, acc, da + 2 * k, db + ((c * kChunkBytes + k * 32) >> 4), idesc, 1);
+              }
+            }
+            umma_commit_if(go, &k_empty[ring.stage]);
+            ring = after;
+          }
+          if (!ok) break;
+          umma_commit_if(go, &acc_full[a]);
+          ++g;
+          room = g < 2 || mbar_try_wait(&acc_free[g & 1], ((g >> 1) + 1) & 1);
         }
-        if (!ok) break;
-        umma_commit_if(go, &acc_full[a]);
-        ++g;
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_free[item & 1]);
     }
   } else {
-    // ================================ query rows, then epilogue: thread = key ========================
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    // ================================ heads to tensor memory; epilogue ==============================
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;   // this thread's head and half of the keys
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const float inv_h = 1.f / static_cast<float>(p.H);
-    int g = 0;
-    bool ok = run;
-    for (int pass = 0; pass < passes; ++pass) {   // (also when a wait has given up: the barriers below count every thread)
-      const int h0 = pass * kHeads, heads = min(kHeads, p.H - h0);
-      // (the last pass's MMAs are done: their accumulators have been read below)
-      const T* q = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(bt) * p.H + h0) * p.D;
-      for (int i = tid; i < sh.chunks * sh.n * 8; i += 128) {
-        const int unit = i & 7, row = (i >> 3) % sh.n, ch = (i >> 3) / sh.n;
-        const bool copy = row < heads && ch * 64 + unit * 8 < p.D;
-        cp_async16(sQ + ch * q_chunk + sw128_offset(row, unit), copy ? q + static_cast<int64_t>(row) * p.D + ch * 64 + unit * 8 : q, copy ? 16u : 0u);
-      }
-      cp_async_arrive_noinc(q_full);
-      named_bar_sync(1, 128);   // the last pass's normalisers have been used
-      {
-        // a head without any key has lse = -inf: no weight (neither have the rows that pad the heads)
-        const float l = tid < heads ? p.lse[static_cast<int64_t>(bt) * p.H + h0 + tid] : INFINITY;
-        s_lse[tid] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
-      }
-      named_bar_sync(1, 128);
-      for (int tile = 0; ok && tile < tiles; ++tile) {
-        const int slot = tile * kKeys + tid;
-        float sum = 0.f;
-        if (any_key(tile)) {
-          const int a = g & 1;
-          if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[a], (g >> 1) & 1, p.status))) { ok = false; break; }
-          tc_fence_after();
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int c0 = 0; c0 < sh.n; c0 += 16) {
-            uint32_t v[16];
-            tmem_ld16(tmem_base + a * kHeads + c0 + lane_base, v);
-            tmem_wait_ld();
-            const float4* l4 = reinterpret_cast<const float4*>(s_lse + c0);
+    Ring ring;
+    // The heads of a pass: the two halves take alternate chunks out of the ring.  All MMAs that read the heads before are done: every
+    // warp has seen the commit of the last of them.
+    auto move_heads = [&](bool go) {
+      for (int part = 0; part < sh.parts; ++part) {
+        go = go && wait(&k_full[ring.stage], ring.phase);
+#pragma unroll 1
+        for (int c = 0; c < kPerStage; ++c) {
+          const int ch = part * kPerStage + c;
+          if ((ch & 1) != half || ch >= sh.chunks) continue;
+          const uint32_t src = sK + ring.stage * kStageBytes + c * kChunkBytes;
+          uint32_t w[32];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float4 l = l4[j];
-              part[0] += exp2f(fmaf(__uint_as_float(v[4 * j]), p.scale_log2, -l.x));
-              part[1] += exp2f(fmaf(__uint_as_float(v[4 * j + 1]), p.scale_log2, -l.y));
-              part[2] += exp2f(fmaf(__uint_as_float(v[4 * j + 2]), p.scale_log2, -l.z));
-              part[3] += exp2f(fmaf(__uint_as_float(v[4 * j + 3]), p.scale_log2, -l.w));
-            }
+          for (int j = 0; j < 8; ++j) {
+            const uint4 v = ld_shared_v4(src + sw128_offset(row, j));
+            w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
           }
-          tc_fence_before();
-          mbar_arrive(&acc_empty[a]);
-          ++g;
-          sum = ((s_bits[slot >> 5] >> (slot & 31)) & 1u) ? ((part[0] + part[1]) + (part[2] + part[3])) * inv_h : 0.f;
+          if (ch < kTmemChunks) {
+            if (go) tmem_st32(tmem_base + lane_base + ch * 32, w);
+          } else {
+            const uint32_t dst = sQ + (ch - kTmemChunks) * kChunkBytes;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) st_shared_v4(dst + sw128_offset(row, j), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          }
         }
-        if (slot < p.topk) out[slot] = pass ? out[slot] + sum : sum;
+        named_bar_sync(1, kEpilogueWarps * 32);   // all warps have read the stage
+        if (tid == 0 && go) mbar_arrive(&k_empty[ring.stage]);
+        ring.next(sh.stages);
       }
+      tmem_wait_st();
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && go) mbar_arrive(q_ready);
+      return go;
+    };
+    auto lse_of = [&](int bt, int pass) {   // in log2 units; a head without any key has lse = -inf: no weight (neither have the rows that pad the heads)
+      const int h = pass * kHeads + row;
+      const float l = h < p.H ? __ldg(p.lse + static_cast<int64_t>(bt) * p.H + h) : INFINITY;
+      return l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+    };
+    int g = 0;
+    bool moved = false;      // the next pass's heads are in place already
+    float lse = 0.f, next_lse = 0.f;
+    // (Every warp of the group takes the same turns through these loops, also when a wait has given up: the barriers inside count
+    // them all.  Whether a list can be trusted is agreed on.)
+    for (int item = 0; item < items; ++item) {
+      ok = bar_and(1, kEpilogueWarps * 32, ok && wait(&list_full[item & 1], (item >> 1) & 1));
+      if (!ok) break;
+      const uint32_t* bits = bits_of(item);
+      const int bt = query_of(item);
+      float* out = weights + static_cast<int64_t>(bt) * p.topk;
+      if (!bits[kMaxWords]) {
+        for (int i = tid; i < p.topk; i += kEpilogueWarps * 32) out[i] = 0.f;
+      } else {
+        const uint8_t* list = tiles_of(item);
+        const int count = bits[kMaxWords];
+        // tiles without a key
+        for (int tile = 0; tile < tiles; ++tile) {
+          const int slot = tile * kKeys + tid;
+          if (tid < kKeys && slot < p.topk && !(bits[4 * tile] | bits[4 * tile + 1] | bits[4 * tile + 2] | bits[4 * tile + 3])) out[slot] = 0.f;
+        }
+        for (int pass = 0; pass < passes; ++pass) {
+          if (!moved) {
+            next_lse = lse_of(bt, pass);
+            ok = move_heads(ok);
+          }
+          moved = false;
+          lse = next_lse;
+          for (int i = 0; i < count; ++i) {
+            const int slot = list[i] * kKeys + tid;   // (of the combining threads, tid < 128)
+            const int a = g & 1;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[a], (g >> 1) & 1, p.status));
+            ring.skip(sh.parts, sh.stages);   // this tile's slots were the MMAs'
+            if (i + 1 == count) {               // no MMA reads these heads any more: the next ones take their place before the epilogue
+              if (pass + 1 < passes) {
+                next_lse = lse_of(bt, pass + 1);
+                ok = move_heads(ok);
+                moved = true;
+              } else if (item + 1 < items) {
+                ok = bar_and(1, kEpilogueWarps * 32, ok && wait(&list_full[(item + 1) & 1], ((item + 1) >> 1) & 1));
+                if (ok && bits_of(item + 1)[kMaxWords]) {
+                  next_lse = lse_of(query_of(item + 1), 0);
+                  ok = move_heads(ok);
+                  moved = true;
+                }
+              }
+            }
+            tc_fence_after();
+            float* part = s_part + (a * 4 + quarter) * kKeys + half * 64;
+#pragma unroll
+            for (int grp = 0; grp < 2; ++grp) {
+              uint32_t v[32];
+              if (ok) {
+                tmem_ld32(tmem_base + kColS + a * kKeys + half * 64 + grp * 32 + lane_base, v);
+                tmem_wait_ld();
+              }
+              if (grp == 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_free[a]);
+              }
+              float e[32];
+#pragma unroll
+              for (int k = 0; k < 32; ++k) e[k] = exp2f(fmaf(__uint_as_float(v[k]), p.scale_log2, -lse));
+              // over the heads of this quarter: lane l ends with the sum for key l of the group
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) {
+                const bool upper = lane & o;
+#pragma unroll
+                for (int k = 0; k < o; ++k) {
+                  const float give = upper ? e[k] : e[k + o], mine = upper ? e[k + o] : e[k];
+                  e[k] = mine + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+              }
+              part[grp * 32 + lane] = e[0];
+            }
+            named_bar_sync(1, kEpilogueWarps * 32);
+            if (tid < kKeys && slot < p.topk && ok) {
+              const float* q4 = s_part + a * 4 * kKeys + tid;
+              const float sum = ((bits[slot >> 5] >> (slot & 31)) & 1u) ? ((q4[0] + q4[kKeys]) + (q4[2 * kKeys] + q4[3 * kKeys])) * inv_h : 0.f;
+              out[slot] = pass ? out[slot] + sum : sum;
+            }
+            ++g;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_free[item & 1]);
     }
-    cp_async_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -218,15 +433,14 @@ int launch_sparse_mla_key_weights(const FwdParams& p, float* weights, bool bf16,
   if (e != cudaSuccess) return static_cast<int>(e);
   kw::Shape sh;
   sh.chunks = (p.D + 63) / 64;
-  sh.n = p.H >= kw::kHeads ? kw::kHeads : (p.H + 15) / 16 * 16;
-  // as many stages as shared memory holds beside the heads (576 dims: 128 heads 5, 64 heads 9)
-  const uint32_t q_bytes = static_cast<uint32_t>(sh.chunks) * sh.n * 128;
-  sh.stages = static_cast<int>((kw::kMaxSmem - kw::kFixedBytes - q_bytes) / kw::kChunkBytes);
-  if (sh.stages > kw::kMaxStages) sh.stages = kw::kMaxStages;
-  const int smem = static_cast<int>(q_bytes + sh.stages * kw::kChunkBytes + kw::kFixedBytes);
+  sh.parts = (sh.chunks + kw::kPerStage - 1) / kw::kPerStage;
+  sh.smem_chunks = sh.chunks > kw::kTmemChunks ? sh.chunks - kw::kTmemChunks : 0;
+  sh.stages = static_cast<int>((kw::kMaxSmem - kw::kFixedBytes - sh.smem_chunks * kw::kChunkBytes) / kw::kStageBytes);   // 4; 640 dims: 3
+  const int smem = static_cast<int>(sh.smem_chunks * kw::kChunkBytes + sh.stages * kw::kStageBytes + kw::kFixedBytes);
   auto kern = bf16 ? sparse_mla_key_weights_kernel<true> : sparse_mla_key_weights_kernel<false>;
   if ((e = ensure_dynamic_smem(kern, dev, smem)) != cudaSuccess) return static_cast<int>(e);
-  kern<<<static_cast<unsigned>(p.B) * p.S, kw::kThreads, smem, stream>>>(p, weights, sh);
+  const long long n = static_cast<long long>(p.B) * p.S;
+  kern<<<static_cast<unsigned>(n < sms ? n : sms), kw::kThreads, smem, stream>>>(p, weights, sh);
   return static_cast<int>(cudaGetLastError());
 }
 
