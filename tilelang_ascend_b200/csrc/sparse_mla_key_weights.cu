@@ -13,7 +13,9 @@
 // Persistent CTAs, one per SM, long (late) queries first.  A query's heads ride the ring ahead of its keys and are moved to
 // tensor memory by the epilogue warps as soon as the last MMAs of the query before are done, so that the gather never stops.
 // Warps: 8 epilogue (quarter of the heads x half of the keys), 8 gather, the MMA issuer, and one that reads the next query's list.
-// The sum over heads goes over the lanes by halving exchanges (31 shuffles for 32 keys), then over the four quarters.
+// Shuffles, copies and barriers share one pipe, so the sum over heads uses few: a thread takes four heads of the same keys out of
+// tensor memory and seven shuffles join 32 keys over a warp (one head per thread: 31; with that the epilogue took 3600 of the 2304
+// clocks that a tile's MMAs take, and the copies waited behind it: 848 us).
 #include <type_traits>
 
 #include "fwd_common.cuh"
@@ -205,8 +207,8 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
           const int slot0 = list[i] * kKeys + row0;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const int slot = slot0 + 4 * k;
-            row[k] = (bits[slot >> 5] >> (slot & 31)) & 1u ? __ldg(c.idx_row + slot) : -1;
+            const int slot = slot0 + 4 * k, idx = slot < p.topk ? __ldg(c.idx_row + slot) : -1;
+            row[k] = index_valid(c, idx) ? idx : -1;
           }
         };
         for (int pass = 0; ok && pass < passes; ++pass) {
@@ -234,29 +236,38 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
     // ================================ MMA issuer (converged, one elected lane issues) ===============
     constexpr uint32_t idesc = make_idesc_f16(kBF16, kHeads, kKeys, 0, 0);
     const uint32_t go = elect_one_lane();
+    // (a reduction's result is known to be the same in all lanes, a word from shared memory is not: the operands of an MMA are uniform
+    // registers, and moving them there one by one cost more than the MMA)
+    const uint32_t tmem = __reduce_or_sync(0xffffffffu, tmem_base);
     Ring ring;
     int g = 0, loads = 0;   // tiles and passes so far
-    // A barrier is looked at ahead of the work before it (the answer takes 200 clocks on this busy shared memory); `yes`: it was complete.
-    auto ready = [&](bool yes, uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, yes) || wait(bar, parity); };
+    // The next stage and the next accumulator are looked at in the middle of a stage's MMAs (the answer of a barrier takes 200 clocks on
+    // this busy shared memory, the fence 50 to 100); `yes`: it was complete, and what it announces has been fenced.
+    auto look = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) != 0; };
+    auto fence = [&]() {
+      fence_proxy_async_smem();   // the rows were written by cp.async of other threads
+      tc_fence_after();
+    };
     for (int item = 0; ok && item < items; ++item) {
       if (!wait(&list_full[item & 1], (item >> 1) & 1)) { ok = false; break; }
-      const int count = bits_of(item)[kMaxWords];
+      const int count = __reduce_or_sync(0xffffffffu, bits_of(item)[kMaxWords]);
       for (int pass = 0; ok && count && pass < passes; ++pass) {
         ring.skip(sh.parts, sh.stages);   // the heads' slots are the epilogue warps'
         if (!wait(q_ready, loads & 1)) { ok = false; break; }
         ++loads;
-        bool full = mbar_try_wait(&k_full[ring.stage], ring.phase), room = g < 2 || mbar_try_wait(&acc_free[g & 1], ((g >> 1) + 1) & 1);
+        bool full = false, room = g < 2;
         for (int i = 0; ok && i < count; ++i) {
           const int a = g & 1;
-          if (g >= 2 && !ready(room, &acc_free[a], ((g >> 1) + 1) & 1)) { ok = false; break; }
-          const uint32_t acc = tmem_base + kColS + a * kKeys;
+          if (!room && !wait(&acc_free[a], ((g >> 1) + 1) & 1)) { ok = false; break; }
+          const uint32_t acc = tmem + kColS + a * kKeys;
+          room = g < 1;   // the tile after this one
           for (int part = 0; part < sh.parts; ++part) {
-            if (!ready(full, &k_full[ring.stage], ring.phase)) { ok = false; break; }
+            if (!full) {
+              if (!wait(&k_full[ring.stage], ring.phase)) { ok = false; break; }
+              fence();
+            }
             Ring after = ring;
             after.next(sh.stages);
-            full = mbar_try_wait(&k_full[after.stage], after.phase);
-            fence_proxy_async_smem();   // the rows were written by cp.async of other threads
-            tc_fence_after();
             const uint64_t db = make_smem_desc(sK + ring.stage * kStageBytes, 16, 1024, kSwizzle128B);
 #pragma unroll
             for (int c = 0; c < kPerStage; ++c) {
@@ -264,11 +275,17 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
               if (ch < kTmemChunks && ch < sh.chunks) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  umma_ts_if(go, acc, tmem_base + (ch * 4 + k) * 8, db + ((c * kChunkBytes + k * 32) >> 4), idesc, (ch | k) != 0);
+                  umma_ts_if(go, acc, tmem + (ch * 4 + k) * 8, db + ((c * kChunkBytes + k * 32) >> 4), idesc, (ch | k) != 0);
               } else if (ch < sh.chunks) {
                 const uint64_t da = make_smem_desc(sQ + (ch - kTmemChunks) * kChunkBytes, 16, 1024, kSwizzle128B);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) umma_ss_if(go, acc, da + 2 * k, db + ((c * kChunkBytes + k * 32) >> 4), idesc, 1);
+              }
+              if (c == 1) {
+                // (the last stage of a pass is followed by heads, which are not this warp's)
+                full = (part + 1 < sh.parts || i + 1 < count) && look(&k_full[after.stage], after.phase);
+                if (part + 1 == sh.parts && !room) room = look(&acc_free[(g + 1) & 1], (((g + 1) >> 1) + 1) & 1);
+                if (full) fence();
               }
             }
             umma_commit_if(go, &k_empty[ring.stage]);
@@ -277,7 +294,6 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
           if (!ok) break;
           umma_commit_if(go, &acc_full[a]);
           ++g;
-          room = g < 2 || mbar_try_wait(&acc_free[g & 1], ((g >> 1) + 1) & 1);
         }
       }
       __syncwarp();
@@ -324,14 +340,19 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
       if (lane == 0 && go) mbar_arrive(q_ready);
       return go;
     };
-    auto lse_of = [&](int bt, int pass) {   // in log2 units; a head without any key has lse = -inf: no weight (neither have the rows that pad the heads)
-      const int h = pass * kHeads + row;
-      const float l = h < p.H ? __ldg(p.lse + static_cast<int64_t>(bt) * p.H + h) : INFINITY;
-      return l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+    // Normalisers of this thread's four heads, in log2 units; a head without any key has lse = -inf: no weight (neither have the rows
+    // that pad the heads).
+    auto load_lse = [&](int bt, int pass, float (&to)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int h = pass * kHeads + quarter * 32 + (lane >> 2) + 8 * i;
+        const float l = h < p.H ? __ldg(p.lse + static_cast<int64_t>(bt) * p.H + h) : INFINITY;
+        to[i] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+      }
     };
     int g = 0;
     bool moved = false;      // the next pass's heads are in place already
-    float lse = 0.f, next_lse = 0.f;
+    float lse[4] = {0.f, 0.f, 0.f, 0.f}, next_lse[4] = {0.f, 0.f, 0.f, 0.f};
     // (Every warp of the group takes the same turns through these loops, also when a wait has given up: the barriers inside count
     // them all.  Whether a list can be trusted is agreed on.)
     for (int item = 0; item < items; ++item) {
@@ -352,11 +373,12 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
         }
         for (int pass = 0; pass < passes; ++pass) {
           if (!moved) {
-            next_lse = lse_of(bt, pass);
+            load_lse(bt, pass, next_lse);
             ok = move_heads(ok);
           }
           moved = false;
-          lse = next_lse;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) lse[k] = next_lse[k];
           for (int i = 0; i < count; ++i) {
             const int slot = list[i] * kKeys + tid;   // (of the combining threads, tid < 128)
             const int a = g & 1;
@@ -364,25 +386,29 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
             ring.skip(sh.parts, sh.stages);   // this tile's slots were the MMAs'
             if (i + 1 == count) {               // no MMA reads these heads any more: the next ones take their place before the epilogue
               if (pass + 1 < passes) {
-                next_lse = lse_of(bt, pass + 1);
+                load_lse(bt, pass + 1, next_lse);
                 ok = move_heads(ok);
                 moved = true;
               } else if (item + 1 < items) {
                 ok = bar_and(1, kEpilogueWarps * 32, ok && wait(&list_full[(item + 1) & 1], ((item + 1) >> 1) & 1));
                 if (ok && bits_of(item + 1)[kMaxWords]) {
-                  next_lse = lse_of(query_of(item + 1), 0);
+                  load_lse(query_of(item + 1), 0, next_lse);
                   ok = move_heads(ok);
                   moved = true;
                 }
               }
             }
             tc_fence_after();
+            // 32 keys at a time: this thread has two keys of every eight for four heads of its quarter, adds those up itself and ends, after
+            // three halving exchanges with the lanes of the other heads, with the quarter's sum for one key.
             float* part = s_part + (a * 4 + quarter) * kKeys + half * 64;
 #pragma unroll
             for (int grp = 0; grp < 2; ++grp) {
-              uint32_t v[32];
+              uint32_t lo[16], hi[16];
               if (ok) {
-                tmem_ld32(tmem_base + kColS + a * kKeys + half * 64 + grp * 32 + lane_base, v);
+                const uint32_t from = tmem_base + kColS + a * kKeys + half * 64 + grp * 32 + lane_base;
+                tmem_ld_16x32(from, lo);
+                tmem_ld_16x32(from + (16u << 16), hi);
                 tmem_wait_ld();
               }
               if (grp == 1) {
@@ -390,20 +416,23 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&acc_free[a]);
               }
-              float e[32];
+              float e[8];
 #pragma unroll
-              for (int k = 0; k < 32; ++k) e[k] = exp2f(fmaf(__uint_as_float(v[k]), p.scale_log2, -lse));
-              // over the heads of this quarter: lane l ends with the sum for key l of the group
+              for (int k = 0; k < 8; ++k) {
+                const int r = 4 * (k >> 1) + (k & 1);
+                e[k] = (exp2f(fmaf(__uint_as_float(lo[r]), p.scale_log2, -lse[0])) + exp2f(fmaf(__uint_as_float(lo[r + 2]), p.scale_log2, -lse[1]))) +
+                       (exp2f(fmaf(__uint_as_float(hi[r]), p.scale_log2, -lse[2])) + exp2f(fmaf(__uint_as_float(hi[r + 2]), p.scale_log2, -lse[3])));
+              }
 #pragma unroll
-              for (int o = 16; o > 0; o >>= 1) {
+              for (int o = 16; o >= 4; o >>= 1) {
                 const bool upper = lane & o;
 #pragma unroll
-                for (int k = 0; k < o; ++k) {
-                  const float give = upper ? e[k] : e[k + o], mine = upper ? e[k + o] : e[k];
+                for (int k = 0; k < o / 4; ++k) {
+                  const float give = upper ? e[k] : e[k + o / 4], mine = upper ? e[k + o / 4] : e[k];
                   e[k] = mine + __shfl_xor_sync(0xffffffffu, give, o);
                 }
               }
-              part[grp * 32 + lane] = e[0];
+              part[grp * 32 + 8 * (lane >> 3) + 2 * (lane & 3) + ((lane >> 2) & 1)] = e[0];
             }
             named_bar_sync(1, kEpilogueWarps * 32);
             if (tid < kKeys && slot < p.topk && ok) {
