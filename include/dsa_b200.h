@@ -336,10 +336,12 @@ int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const vo
  * [0, V) and the student's logit there is not -inf; p = the teacher's entries (weights, or exp(logit / temperature) when
  * teacher_logits) over their sum, s = softmax(student / temperature) over the participating entries, or over the whole row when
  * over_row: loss [rows] fp32 = sum p (log p - log s), 0 for rows without teacher weight.  stats [rows, 4] fp32 (16-byte aligned) is
- * what the backward needs.  dtypes: 0 bfloat16, 1 float16, 2 float32.  No reference counterpart. */
+ * what the backward needs.  workspace: dsa_topk_distillation_workspace_bytes (0: NULL).  dtypes: 0 bfloat16, 1 float16, 2 float32.
+ * No reference counterpart. */
+size_t dsa_topk_distillation_workspace_bytes(int64_t rows, int32_t V, int32_t over_row, int32_t listed);
 int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,
                           const int32_t* indices, float* loss, float* stats, int64_t rows, int32_t V, int32_t K, int32_t over_row,
-                          int32_t teacher_logits, float temperature, void* stream);
+                          int32_t teacher_logits, float temperature, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Its gradient: grad [rows] fp32, d_student [rows, V] contiguous (the student's type), every column written.  A column that a row
  * lists more than once gets the sum of its entries (of three or more in no fixed order). */

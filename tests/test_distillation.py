@@ -232,5 +232,5 @@ def test_refusals():
 def test_c_entry_refuses_before_any_cuda_call():
     from tilelang_ascend_b200 import _lib
     lib = _lib.load()
-    assert lib.dsa_topk_distillation(None, 2, 4, None, 2, None, None, None, 1, 4, 4, 0, 0, 1.0, None) != 0
+    assert lib.dsa_topk_distillation(None, 2, 4, None, 2, None, None, None, 1, 4, 4, 0, 0, 1.0, None, 0, None) != 0
     assert lib.dsa_topk_distillation_bwd(None, 2, 4, None, 2, None, None, None, None, 1, 4, 4, 0, 0, 1.0, None) != 0

@@ -93,8 +93,9 @@ SIGNATURES = {
     "dsa_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int32]),
     "dsa_norm_rope_bwd": (c_int32, [ctypes.POINTER(RopeGrads), ctypes.POINTER(RopeGrads), c_void_p, c_int32, c_void_p] + [c_int32] * 7
                           + [c_float, c_float, c_void_p, c_size_t, c_int32, c_void_p]),
+    "dsa_topk_distillation_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
     "dsa_topk_distillation": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64] + [c_int32] * 4
-                              + [c_float, c_void_p]),
+                              + [c_float, c_void_p, c_size_t, c_void_p]),
     "dsa_topk_distillation_bwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64]
                                   + [c_int32] * 4 + [c_float, c_void_p]),
     "dsa_sparse_mla_key_weights": (c_int32, [c_void_p] * 5 + [c_int32] * 6 + [c_float, c_int32, c_int32, c_int32, c_void_p]),

@@ -633,13 +633,20 @@ int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const vo
   return err ? fail_cuda("norm_rope_bwd launch", err) : 0;
 }
 
+size_t dsa_topk_distillation_workspace_bytes(int64_t rows, int32_t V, int32_t over_row, int32_t listed) {
+  return rows > 0 && V > 0 ? dsa::distill_workspace_bytes(rows, V, over_row, listed != 0) : 0;
+}
+
 int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype, const int32_t* indices,
                           float* loss, float* stats, int64_t rows, int32_t V, int32_t K, int32_t over_row, int32_t teacher_logits, float temperature,
-                          void* stream) {
+                          void* workspace, size_t workspace_bytes, void* stream) {
   dsa::DistillParams p;
   if (!loss) return fail("null output pointer");
   if (fill_distill(&p, student, student_dtype, row_stride, teacher, teacher_dtype, indices, stats, rows, V, K, over_row, teacher_logits, temperature)) return 1;
   p.loss = loss;
+  const size_t need = dsa::distill_workspace_bytes(rows, V, over_row, indices != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return fail("workspace too small (see dsa_topk_distillation_workspace_bytes)");
+  p.partials = need ? static_cast<float*>(workspace) : nullptr;
   int err = dsa::launch_distill_fwd(p, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("topk_distillation launch", err) : 0;
 }

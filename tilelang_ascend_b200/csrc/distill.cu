@@ -20,6 +20,7 @@
 
 #include "distill.h"
 #include "launch_util.h"
+#include "ptx.cuh"
 
 namespace dsa {
 
@@ -27,6 +28,7 @@ namespace dt {
 constexpr float kLowest = -3.402823466e38f, kLn2 = 0.6931471805599453f;
 constexpr int kChunk = 8192;         // columns of a backward block with indices: 32 KB of sums
 constexpr int kListedThreads = 512;
+constexpr int kPartChunks = 4;       // chunks of a part of the forward
 constexpr int kPerThread = kChunk / kListedThreads;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -172,12 +174,15 @@ struct Online {
 struct List {
   Online z;
   float tm = kLowest, W = 0.f, A = 0.f;
-  __device__ __forceinline__ void add(const DistillParams& p, const float (&zs)[4], const float (&ts)[4]) {
+  template <int N>
+  __device__ __forceinline__ void add(const DistillParams& p, const float (&zs)[N], const float (&ts)[N]) {
     const float before = z.m;
     z.add(zs, p.exp_scale);
     if (z.m > before && W != 0.f) A += W * ((z.m - before) * p.inv_T);
     if (p.teacher_logits) {
-      const float top = fmaxf(fmaxf(ts[0], ts[1]), fmaxf(ts[2], ts[3]));
+      float top = ts[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top = fmaxf(top, ts[i]);
       if (top > tm) {
         if (W != 0.f) {
           const float f = exp_from(tm, top, p.exp_scale);
@@ -188,7 +193,7 @@ struct List {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       const float w = p.teacher_logits ? exp_from(ts[i], tm, p.exp_scale) : ts[i];
       if (w != 0.f) {   // (also keeps -inf out of a product with 0)
         const float log_w = p.teacher_logits ? (ts[i] - tm) * p.inv_T : ln_of(w);
@@ -198,6 +203,77 @@ struct List {
     }
   }
 };
+
+// sum = {S, W, A} of a thread or part with the row maximum m, A relative to the list maximum zm and teacher maximum tm: made relative
+// to the maxima `top` = {row, teacher} instead.
+__device__ __forceinline__ void rebase(const DistillParams& p, float (&sum)[3], float m, float zm, float tm, const float (&top)[2]) {
+  sum[0] *= exp_from(m, top[0], p.exp_scale);
+  if (sum[1] != 0.f) {
+    sum[2] += sum[1] * ((top[0] - zm) * p.inv_T);
+    if (p.teacher_logits) {
+      const float f = exp_from(tm, top[1], p.exp_scale);
+      sum[2] = f > 0.f ? f * (sum[2] + sum[1] * ((tm - top[1]) * p.inv_T)) : 0.f;
+      sum[1] *= f;
+    }
+  }
+}
+// Loss of a row from its joined sums, and what the backward needs of it.
+__device__ __forceinline__ void finish_row(const DistillParams& p, int64_t r, const float (&top)[2], const float (&sum)[3]) {
+  const float W = sum[1];
+  const bool active = !(W == 0.f);   // (NaN: the loss says so)
+  p.loss[r] = active ? sum[2] / W - logf(W) + logf(sum[0]) : 0.f;
+  // for the backward: maximum and reciprocal sum of the student; of the teacher the maximum of the logits, or a factor that keeps
+  // the weights' reciprocal sum finite, and that reciprocal (0: no gradient)
+  const float factor = p.teacher_logits ? 1.f : (W < 0x1p-100f ? 0x1p100f : 1.f);
+  reinterpret_cast<float4*>(p.stats)[r] =
+      make_float4(top[0], active ? 1.f / sum[0] : 0.f, p.teacher_logits ? top[1] : factor, active ? 1.f / (W * factor) : 0.f);
+}
+
+// A block's kChunk columns in registers: 16-byte units (kWide) or single elements, kListedThreads apart.
+template <typename T, bool kWide>
+struct Columns {
+  static constexpr int kN = kWide ? Vec<T>::kN : 1, kUnits = kPerThread / kN;
+  Vec<T> wide[kWide ? kUnits : 1];
+  float narrow[kWide ? 1 : kUnits];
+  __device__ __forceinline__ void load(const T* src, int n, int tid) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = (tid + u * kListedThreads) * kN;
+      if (c < n) {
+        if constexpr (kWide) wide[u].load(src + c);
+        else narrow[u] = to_f(src[c]);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int u, int k) const {
+    if constexpr (kWide) return wide[u].get(k);
+    else return narrow[u];
+  }
+};
+
+// A thread's first kAhead indices of a list, asked for before anything else; then f(column - c0, j) for those of its entries whose column
+// lies in [c0, c0 + n).
+constexpr int kAhead = 4;
+__device__ __forceinline__ void first_indices(const DistillParams& p, int64_t r, int tid, int (&idx)[kAhead]) {
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int j = tid + i * kListedThreads;
+    idx[i] = j < p.K ? __ldg(p.indices + r * p.K + j) : -1;
+  }
+}
+template <typename F>
+__device__ __forceinline__ void for_listed(const DistillParams& p, int64_t r, int tid, const int (&idx)[kAhead], int c0, int n, F f) {
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int c = idx[i] - c0;
+    if (idx[i] >= 0 && c >= 0 && c < n) f(c, tid + i * kListedThreads);
+  }
+  for (int j = tid + kAhead * kListedThreads; j < p.K; j += kListedThreads) {
+    const int k = __ldg(p.indices + r * p.K + j), c = k - c0;
+    if (k >= 0 && c >= 0 && c < n) f(c, j);
+  }
+}
+constexpr int kPartial = 5;   // floats a part leaves for the join
 }  // namespace dt
 
 // -------------------------------------------------------------------------------------------------
@@ -252,27 +328,118 @@ __global__ void __launch_bounds__(kThreads, kBlocks) distill_fwd_kernel(const __
   }
   float top[2] = {all.m, list.tm};
   block_reduce<kThreads>(top, s_max, Max());
-  // to the block's maxima
-  float sum[3] = {all.s * exp_from(all.m, top[0], p.exp_scale), list.W, list.A};
-  if (list.W != 0.f) {
-    sum[2] += list.W * ((top[0] - list.z.m) * p.inv_T);
-    if (p.teacher_logits) {
-      const float f = exp_from(list.tm, top[1], p.exp_scale);
-      sum[2] = f > 0.f ? f * (sum[2] + list.W * ((list.tm - top[1]) * p.inv_T)) : 0.f;
-      sum[1] *= f;
-    }
-  }
+  float sum[3] = {all.s, list.W, list.A};
+  rebase(p, sum, all.m, list.z.m, list.tm, top);
   block_reduce<kThreads>(sum, s_sum, Sum());
-  if (tid == 0) {
-    const float W = sum[1];
-    const bool active = !(W == 0.f);   // (NaN: the loss says so)
-    p.loss[r] = active ? sum[2] / W - logf(W) + logf(sum[0]) : 0.f;
-    // for the backward: maximum and reciprocal sum of the student; of the teacher the maximum of the logits, or a factor that keeps
-    // the weights' reciprocal sum finite, and that reciprocal (0: no gradient)
-    const float factor = p.teacher_logits ? 1.f : (W < 0x1p-100f ? 0x1p100f : 1.f);
-    reinterpret_cast<float4*>(p.stats)[r] =
-        make_float4(top[0], active ? 1.f / sum[0] : 0.f, p.teacher_logits ? top[1] : factor, active ? 1.f / (W * factor) : 0.f);
+  if (tid == 0) finish_row(p, r, top, sum);
+}
+
+// -------------------------------------------------------------------------------------------------
+// forward of wide rows, in parts: block = (row, kPartChunks chunks of its columns).  A chunk passes through one of two shared-memory
+// buffers, the next one on its way meanwhile, and the listed entries of its columns are looked up there: gathered from global memory,
+// 2048 entries of a row of 131072 cost as much as half of the row (1024 such rows: 141 us; one chunk per block: 147 us).
+// kWide: rows in aligned 16-byte units, copied asynchronously; else element by element.
+// -------------------------------------------------------------------------------------------------
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(dt::kListedThreads) distill_fwd_part_kernel(const __grid_constant__ DistillParams p, const int parts) {
+  using namespace dt;
+  extern __shared__ __align__(16) uint8_t buffers[];   // T [2][kChunk]
+  __shared__ float s_max[kListedThreads / 32][2], s_sum[kListedThreads / 32][3];
+  constexpr int kN = kWide ? Vec<T>::kN : 1;
+  const int64_t r = blockIdx.x / parts;
+  const int first = static_cast<int>(blockIdx.x - r * parts) * kPartChunks * kChunk, cols = min(p.V - first, kPartChunks * kChunk);
+  const int tid = threadIdx.x;
+  const T* src = static_cast<const T*>(p.student) + r * p.row_stride + first;
+  int idx[kAhead];
+  first_indices(p, r, tid, idx);
+  auto buffer = [&](int i) { return reinterpret_cast<T*>(buffers) + (i & 1) * kChunk; };
+  auto fetch = [&](int i) {
+    T* to = buffer(i);
+    const T* from = src + i * kChunk;
+    const int n = min(cols - i * kChunk, kChunk);
+    for (int c = tid * kN; c < n; c += kListedThreads * kN) {
+      if constexpr (kWide) cp_async16(smem_u32(to + c), from + c, 16u);
+      else to[c] = from[c];
+    }
+    cp_async_commit();
+  };
+  Online all;
+  List list;
+  const int chunks = (cols + kChunk - 1) / kChunk;
+  fetch(0);
+  for (int i = 0; i < chunks; ++i) {
+    if (i + 1 < chunks) {
+      fetch(i + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    const T* zs = buffer(i);
+    const int n = min(cols - i * kChunk, kChunk);
+    for (int c = tid * kN; c < n; c += kListedThreads * kN) {
+      float z[kN];
+      if constexpr (kWide) {
+        Vec<T> v;
+        v.raw = *reinterpret_cast<const uint4*>(zs + c);
+#pragma unroll
+        for (int k = 0; k < kN; ++k) z[k] = v.get(k);
+      } else {
+        z[0] = to_f(zs[c]);
+      }
+      all.add(z, p.exp_scale);
+    }
+    for_listed(p, r, tid, idx, first + i * kChunk, n, [&](int c, int j) {
+      const float z[1] = {to_f(zs[c])};
+      if (z[0] == -INFINITY) return;
+      float t[1] = {teacher_at(p, r * p.K + j)};
+      if (!p.teacher_logits && t[0] < 0.f) t[0] = 0.f;
+      list.add(p, z, t);
+    });
+    __syncthreads();   // the buffer may be filled again
   }
+  float top[2] = {all.m, list.tm};
+  block_reduce<kListedThreads>(top, s_max, Max());
+  float sum[3] = {all.s, list.W, list.A};
+  rebase(p, sum, all.m, list.z.m, list.tm, top);
+  block_reduce<kListedThreads>(sum, s_sum, Sum());
+  if (tid == 0) {
+    float* out = p.partials + static_cast<int64_t>(blockIdx.x) * kPartial;
+    out[0] = top[0]; out[1] = top[1]; out[2] = sum[0]; out[3] = sum[1]; out[4] = sum[2];
+  }
+}
+
+// The parts of a row together: a warp per row.
+__global__ void __launch_bounds__(128) distill_fwd_join_kernel(const __grid_constant__ DistillParams p, const int parts) {
+  using namespace dt;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= p.rows) return;
+  const float* in = p.partials + r * parts * kPartial;
+  float top[2] = {kLowest, kLowest};
+  for (int i = lane; i < parts; i += 32) {
+    top[0] = fmaxf(top[0], in[i * kPartial]);
+    top[1] = fmaxf(top[1], in[i * kPartial + 1]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+  }
+  float sum[3] = {0.f, 0.f, 0.f};
+  for (int i = lane; i < parts; i += 32) {
+    const float* q = in + i * kPartial;
+    float s[3] = {q[2], q[3], q[4]};
+    rebase(p, s, q[0], q[0], q[1], top);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sum[k] += s[k];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+  }
+  if (lane == 0) finish_row(p, r, top, sum);
 }
 
 namespace dt {
@@ -318,46 +485,33 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const __grid_constant_
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(dt::kListedThreads) distill_bwd_listed_kernel(const __grid_constant__ DistillParams p, const int parts) {
   using namespace dt;
-  __shared__ float acc[kChunk];
+  __shared__ __align__(16) float acc[kChunk];
   constexpr int kN = kWide ? Vec<T>::kN : 1, kUnits = kPerThread / kN;
   const int64_t r = blockIdx.x / parts;
   const int c0 = static_cast<int>(blockIdx.x - r * parts) * kChunk, n = min(p.V - c0, kChunk);
   const int tid = threadIdx.x;
-  const T* row = static_cast<const T*>(p.student) + r * p.row_stride;
-  const T* src = row + c0;
+  const T* src = static_cast<const T*>(p.student) + r * p.row_stride + c0;
   T* out = static_cast<T*>(p.d_student) + r * p.V + c0;
-  // the block's columns travel while the list is looked through
-  Vec<T> wide[kWide ? kUnits : 1];
-  float narrow[kWide ? 1 : kUnits];
-  if (p.over_row) {
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int c = (tid + u * kListedThreads) * kN;
-      if (c < n) {
-        if constexpr (kWide) wide[u].load(src + c);
-        else narrow[u] = to_f(src[c]);
-      }
-    }
-  }
+  int idx[kAhead];
+  first_indices(p, r, tid, idx);
   const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
+  const float grad = __ldg(p.grad + r);
+  Columns<T, kWide> cols;
+  if (p.over_row) cols.load(src, n, tid);   // the block's columns travel while the list is looked through
   const bool active = !(st.w == 0.f);
-  const float g = active ? __ldg(p.grad + r) * p.inv_T : 0.f;
+  const float g = active ? grad * p.inv_T : 0.f;
 #pragma unroll
   for (int i = 0; i < kChunk; i += kListedThreads * 4) *reinterpret_cast<float4*>(acc + i + tid * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  if (active) {
-#pragma unroll 4
-    for (int j = tid; j < p.K; j += kListedThreads) {
-      const int c = __ldg(p.indices + r * p.K + j) - c0;
-      if (c < 0 || c >= n) continue;
+  if (active)
+    for_listed(p, r, tid, idx, c0, n, [&](int c, int j) {
       const float z = to_f(src[c]);
-      if (z == -INFINITY) continue;
+      if (z == -INFINITY) return;
       float t = teacher_at(p, r * p.K + j);
       if (!p.teacher_logits && t < 0.f) t = 0.f;
       const float soft = p.over_row ? 0.f : exp_from(z, st.x, p.exp_scale) * st.y;
       atomicAdd(&acc[c], g * (soft - teacher_p(p, st, t)));
-    }
-  }
+    });
   __syncthreads();
   const float scale = g * st.y;
   auto value = [&](float z, int c) { return p.over_row && active ? fmaf(scale, exp_from(z, st.x, p.exp_scale), acc[c]) : acc[c]; };
@@ -368,10 +522,10 @@ __global__ void __launch_bounds__(dt::kListedThreads) distill_bwd_listed_kernel(
       if constexpr (kWide) {
         Vec<T> o;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) o.set(k, value(wide[u].get(k), c + k));
+        for (int k = 0; k < kN; ++k) o.set(k, value(cols.get(u, k), c + k));
         o.store(out + c);
       } else {
-        out[c] = static_cast<T>(value(narrow[u], c));
+        out[c] = static_cast<T>(value(cols.get(u, 0), c));
       }
     }
   }
@@ -384,25 +538,42 @@ namespace {
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 size_t type_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
 
+int distill_parts(int V) { return (V + dt::kChunk - 1) / dt::kChunk; }
+int forward_parts(int V) { return (distill_parts(V) + dt::kPartChunks - 1) / dt::kPartChunks; }
+// Do all rows (and those of the gradient) come in aligned 16-byte units?
 template <typename T>
-int forward(const DistillParams& p, int sms, cudaStream_t stream) {
+bool wide_rows(const DistillParams& p) {
+  const int n = dt::Vec<T>::kN;
+  return p.V % n == 0 && p.row_stride % n == 0 && aligned(p.student, 16) && (!p.d_student || aligned(p.d_student, 16));
+}
+
+template <typename T>
+int forward(const DistillParams& p, int dev, int sms, cudaStream_t stream) {
   const unsigned rows = static_cast<unsigned>(p.rows);
-  // Whole rows: many of them run side by side in blocks of 256 threads, eight to an SM (1024 rows in blocks of 512 are 1.7 rounds of
-  // the chip); few rows take 1024 threads each.  Lists: 256 threads, 64 where that is four entries each.
-  if (p.over_row && p.V > 4096 && p.rows < 2 * sms) distill_fwd_kernel<T, 1024, 1><<<rows, 1024, 0, stream>>>(p);
+  // Wide rows go in parts.  Other rows: many of them run side by side in blocks of 256 threads, eight to an SM; few rows take 1024
+  // threads each.  Lists: 256 threads, 64 where that is four entries each.
+  if (p.partials) {
+    const int parts = forward_parts(p.V), smem = 2 * dt::kChunk * static_cast<int>(sizeof(T));
+    if (p.rows * parts > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
+    const unsigned grid = rows * static_cast<unsigned>(parts);
+    auto kern = wide_rows<T>(p) ? distill_fwd_part_kernel<T, true> : distill_fwd_part_kernel<T, false>;
+    const cudaError_t e = ensure_dynamic_smem(kern, dev, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    kern<<<grid, dt::kListedThreads, smem, stream>>>(p, parts);
+    distill_fwd_join_kernel<<<(rows + 3) / 4, 128, 0, stream>>>(p, parts);
+  } else if (p.over_row && p.V > 4096 && p.rows < 2 * sms) distill_fwd_kernel<T, 1024, 1><<<rows, 1024, 0, stream>>>(p);
   else if (!p.over_row && p.K <= 256) distill_fwd_kernel<T, 64, 1><<<rows, 64, 0, stream>>>(p);
   else distill_fwd_kernel<T, 256, 8><<<rows, 256, 0, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T>
 int backward(const DistillParams& p, cudaStream_t stream) {
-  const int parts = (p.V + dt::kChunk - 1) / dt::kChunk;
+  const int parts = distill_parts(p.V);
   const int64_t blocks = p.rows * parts;
   if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
   const unsigned grid = static_cast<unsigned>(blocks);
-  const int n = dt::Vec<T>::kN;
   if (!p.indices) distill_bwd_kernel<T><<<grid, 256, 0, stream>>>(p, parts);
-  else if (p.V % n == 0 && p.row_stride % n == 0 && aligned(p.student, 16) && aligned(p.d_student, 16))
+  else if (wide_rows<T>(p))
     distill_bwd_listed_kernel<T, true><<<grid, dt::kListedThreads, 0, stream>>>(p, parts);
   else
     distill_bwd_listed_kernel<T, false><<<grid, dt::kListedThreads, 0, stream>>>(p, parts);
@@ -418,13 +589,18 @@ void finish(DistillParams* p) {
 }
 }  // namespace
 
+// Rows normalised as a whole, wide enough for several parts.
+size_t distill_workspace_bytes(int64_t rows, int V, int over_row, bool listed) {
+  return over_row && listed && V > 2 * dt::kChunk ? static_cast<size_t>(rows) * forward_parts(V) * dt::kPartial * sizeof(float) : 0;
+}
+
 int launch_distill_fwd(DistillParams p, cudaStream_t stream) {
   int dev = 0, sms = 0;
   cudaError_t e = current_device_sms(&dev, &sms);
   if (e != cudaSuccess) return static_cast<int>(e);
   finish(&p);
-  if (p.student_type == kTypeF32) return forward<float>(p, sms, stream);
-  return p.student_type == kTypeBf16 ? forward<__nv_bfloat16>(p, sms, stream) : forward<__half>(p, sms, stream);
+  if (p.student_type == kTypeF32) return forward<float>(p, dev, sms, stream);
+  return p.student_type == kTypeBf16 ? forward<__nv_bfloat16>(p, dev, sms, stream) : forward<__half>(p, dev, sms, stream);
 }
 int launch_distill_bwd(DistillParams p, cudaStream_t stream) {
   finish(&p);

@@ -1,6 +1,7 @@
 // Parameter block of the distillation kernels (distill.cu).
 #pragma once
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace dsa {
@@ -13,6 +14,7 @@ struct DistillParams {
   const int32_t* indices;   // [rows, K] columns of the entries, nullable (K = V: entry j is column j)
   float* loss;              // [rows]
   float* stats;             // [rows, 4], 16-byte aligned
+  float* partials;          // forward: workspace of distill_workspace_bytes, null when that is 0
   const float* grad;        // backward: [rows]
   void* d_student;          // backward: [rows, V], the student's type
   int64_t rows, row_stride;
@@ -22,6 +24,7 @@ struct DistillParams {
   float inv_T, exp_scale;   // 1 / T, log2(e) / T
 };
 
+size_t distill_workspace_bytes(int64_t rows, int V, int over_row, bool listed);
 int launch_distill_fwd(DistillParams p, cudaStream_t stream);
 int launch_distill_bwd(DistillParams p, cudaStream_t stream);
 

@@ -92,8 +92,12 @@ def topk_distillation_raw(student, teacher, indices=None, *, teacher_kind: str =
     loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=dev)
     stats = torch.empty((tail[0], 4), dtype=torch.float32, device=dev)
     if tail[0]:
+        lib = _lib.load()
+        nbytes = lib.dsa_topk_distillation_workspace_bytes(tail[0], tail[1], tail[3], 1) if indices is not None else 0
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         with on_device(dev):
-            _lib.check(_lib.load().dsa_topk_distillation(*_head(student, teacher, indices), loss.data_ptr(), stats.data_ptr(), *tail, raw_stream(dev)))
+            _lib.check(lib.dsa_topk_distillation(*_head(student, teacher, indices), loss.data_ptr(), stats.data_ptr(), *tail, ptr(workspace), nbytes,
+                                                 raw_stream(dev)))
     return loss, stats
 
 
