@@ -534,12 +534,16 @@ void tile(NormRopeParams* p, int which, int rows) {
   sd.tile_tokens = tokens < 1 ? 1 : tokens;
   sd.blocks = ((p->tokens + sd.tile_tokens - 1) / sd.tile_tokens) * ((sd.H + sd.tile_heads - 1) / sd.tile_heads);
 }
-// Rows per block: 64 amortise a block's angles and weights; calls of fewer than four blocks per SM take shorter ones.
+// Rows per block: about 32 KB of them, which amortises a block's angles and weights (4096 tokens, rows of 576 dims: 32 rows 194 us, 128 rows
+// 198; rows of 128 dims, forward + backward: 32 rows 115 us, 128 rows 103); calls whose blocks all fit the chip at once (three per SM) take
+// shorter ones as long as they do (64 tokens x 129 rows of 576 dims: 32 rows 10.4 us, 16 rows -- more blocks than fit -- 14.4).
 void tiles(NormRopeParams* p, int sms) {
-  for (int rows = 64; rows >= 8; rows >>= 1) {
+  int rows = 256;
+  while (rows > 32 && rows * p->D > 16384) rows >>= 1;
+  for (;; rows >>= 1) {
     tile(p, 0, rows);
     tile(p, 1, rows);
-    if (p->side[0].blocks + p->side[1].blocks >= 4 * sms) return;
+    if (rows <= 8 || 2 * (p->side[0].blocks + p->side[1].blocks) > 3 * sms) return;
   }
 }
 int tile_smem(const NormRopeParams& p) {
