@@ -19,7 +19,7 @@ def lists(g, B, S, S_kv, K, holes=True):
     out = torch.full((B, S, 1, K), -1, dtype=torch.int32)
     for b in range(B):
         for s in range(S):
-            n = S_kv - S + 1 + s
+            n = max(S_kv - S + 1 + s, 0)
             keys = torch.randperm(n, generator=g)[:K].to(torch.int32)
             out[b, s, 0, torch.randperm(K, generator=g)[:keys.numel()]] = keys
     if holes and K > 2:
@@ -190,6 +190,57 @@ def test_gradient_of_listed_scores(B, S1, S2, N1, K, exact_signs, dtype):
         off = (got.cpu().double() - want[name]).abs()
         assert got.shape == want[name].shape and bool((off <= bound + 1e-30).all()), f"d{name} off by {float((off - bound).max()):.3g}, largest {float(want[name].abs().max()):.3g}"
     assert dq.dtype == dtype and dk.dtype == torch.float32 and dw.dtype == torch.float32
+
+
+def relative(got, want):
+    return float((got.cpu().double() - want).norm() / want.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S1,S2,N1,K", [(1, 1100, 1100, 64, 600), (2, 1030, 1290, 32, 700), (3, 1400, 1061, 16, 1061), (1, 1024, 4000, 64, 2048)])
+def test_gradient_of_lists_that_hold_most_keys(B, S1, S2, N1, K):
+    """Long lists of many queries, whose gradients are summed tile by tile: against the definition on the GPU in 64 bits, with holes, keys listed twice,
+    queries without keys and padding that was never written."""
+    g = torch.Generator().manual_seed(S1 + N1)
+    query, key, weights, _ = make_indexer(g, B, S1, S2, N1, 4, torch.bfloat16)
+    if S1 <= S2:
+        indices = lists(g, B, S1, S2, K)
+    else:
+        indices = torch.stack([torch.randperm(S2, generator=g)[:K] for _ in range(B * S1)]).view(B, S1, 1, K).to(torch.int32)
+    indices[0, 3, 0, 5:40] = indices[0, 3, 0, 45:80]
+    indices[0, 7:20] = -1
+    query, key, weights, indices = (t.cuda() for t in (query, key, weights, indices))
+    d_values = torch.randn(indices.shape, generator=g).cuda() * 1e-3
+    there = (indices >= 0) & (indices < S2)
+    d_values[~there] = float("nan")
+    # the definition: a dense matrix of gradients (entries of one key add up)
+    dense = torch.zeros((B, S1, S2), dtype=torch.float64, device="cuda")
+    dense.view(B * S1, S2).scatter_add_(1, indices.view(B * S1, K).clamp(0, S2 - 1).long(), torch.where(there, d_values, torch.zeros_like(d_values)).double().view(B * S1, K))
+    want = [torch.zeros(t.shape, dtype=torch.float64) for t in (query, key, weights)]
+    for b in range(B):
+        for s in range(0, S1, 50):
+            q, gr, w = query[b, s:s + 50].double(), dense[b, s:s + 50], weights[b, s:s + 50].double()
+            z = torch.einsum("shd,kd->shk", q, key[b, :, 0].double())
+            want[2][b, s:s + 50] = (z.clamp(min=0) * gr[:, None]).sum(2).cpu()
+            dz = (z > 0) * gr[:, None] * w[:, :, None]
+            want[0][b, s:s + 50] = torch.einsum("shk,kd->shd", dz, key[b, :, 0].double()).cpu()
+            want[1][b, :, 0] += torch.einsum("shk,shd->kd", dz, q).cpu()
+    # norms: dz rounded once (2^-8 at most, of every term), dq once more; dw in fp32
+    bounds = (2 * 2.0 ** -8, 2.0 ** -8, 2.0 ** -18)
+    for name, got, ref, bound in zip("qkw", dsa.lightning_indexer_bwd_raw(query, key, weights, indices, d_values), want, bounds):
+        assert relative(got, ref) <= bound, f"d{name} off by {relative(got, ref):.3g} of its norm"
+        assert name != "q" or not got[0, 7:20].any()
+    check_status()
+    # keys that nobody lists and queries without a list may hold anything
+    taken = torch.zeros((B, S2), dtype=torch.bool, device="cuda")
+    taken.scatter_(1, torch.where(there, indices, torch.zeros_like(indices)).view(B, -1).long(), True)
+    dirty_key, dirty_query = key.clone(), query.clone()
+    if not bool(taken.all()):
+        dirty_key[~taken] = float("nan")
+    dirty_query[0, 9] = INF
+    for name, got, ref, bound in zip("qkw", dsa.lightning_indexer_bwd_raw(dirty_query, dirty_key, weights, indices, d_values), want, bounds):
+        assert relative(got, ref) <= bound, f"d{name} with unwritten padding off by {relative(got, ref):.3g} of its norm"
+    check_status()
 
 
 @pytest.mark.gpu
@@ -400,4 +451,4 @@ def test_c_entries_refuse_before_any_cuda_call():
     from tilelang_ascend_b200 import _lib
     lib = _lib.load()
     assert lib.dsa_sparse_mla_key_weights(None, None, None, None, None, 1, 1, 1, 1, 64, 8, 1.0, 0, 1, 0, None) != 0
-    assert lib.dsa_lightning_indexer_bwd(None, None, None, None, None, None, None, None, 1, 1, 1, 1, 128, 8, 0, None) != 0
+    assert lib.dsa_lightning_indexer_bwd(None, None, None, None, None, None, None, None, 1, 1, 1, 1, 128, 8, 0, None, 0, None) != 0

@@ -99,7 +99,8 @@ SIGNATURES = {
     "dsa_topk_distillation_bwd": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64]
                                   + [c_int32] * 4 + [c_float, c_void_p]),
     "dsa_sparse_mla_key_weights": (c_int32, [c_void_p] * 5 + [c_int32] * 6 + [c_float, c_int32, c_int32, c_int32, c_void_p]),
-    "dsa_lightning_indexer_bwd": (c_int32, [c_void_p] * 8 + [c_int32] * 7 + [c_void_p]),
+    "dsa_lightning_indexer_bwd_workspace_bytes": (c_size_t, [c_int32] * 7),
+    "dsa_lightning_indexer_bwd": (c_int32, [c_void_p] * 8 + [c_int32] * 7 + [c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -676,17 +676,31 @@ int dsa_sparse_mla_key_weights(const void* q, const void* kv, const int32_t* ind
   return err ? fail_cuda("sparse_mla_key_weights launch", err) : 0;
 }
 
+size_t dsa_lightning_indexer_bwd_workspace_bytes(int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype) {
+  if (B <= 0 || S1 <= 0 || S2 <= 0 || N1 <= 0 || K <= 0) return 0;
+  dsa::IndexerBwdParams p{};
+  p.B = B; p.S1 = S1; p.S2 = S2; p.N1 = N1; p.D = D; p.K = K;
+  return dsa::indexer_bwd_workspace_bytes(p, dtype == DSA_DTYPE_BF16);
+}
+
 int dsa_lightning_indexer_bwd(const void* q, const void* k, const float* w, const int32_t* indices, const float* grad, void* d_q, float* d_k, float* d_w,
-                              int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype, void* stream) {
+                              int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype, void* workspace, size_t workspace_bytes,
+                              void* stream) {
   if (!q || !k || !w || !indices || !grad || !d_q || !d_k || !d_w) return fail("null tensor pointer");
   if (!dtype_ok(dtype)) return fail("dtype must be 0 (bfloat16) or 1 (float16)");
   if (B <= 0 || S1 <= 0 || S2 <= 0 || N1 <= 0 || K <= 0) return fail("B, S1, S2, N1 and K must be positive");
   if (static_cast<int64_t>(B) * S1 > 0x3fffffffLL) return fail("B * S1 too large");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k)) & 15u) return fail("q and k must be 16-byte aligned");
-  dsa::IndexerBwdParams p{q, k, w, indices, grad, d_q, d_k, d_w, B, S1, S2, N1, D, K, nullptr};
+  const bool bf16 = dtype == DSA_DTYPE_BF16;
+  dsa::IndexerBwdParams p{q, k, w, indices, grad, d_q, d_k, d_w, B, S1, S2, N1, D, K, nullptr, nullptr};
   if (!dsa::indexer_bwd_supported(p)) return fail("the indexer's backward needs D = 128, at most 64 heads and lists of at most 8192 keys");
+  const size_t need = dsa::indexer_bwd_workspace_bytes(p, bf16);
+  if (need && (!workspace || workspace_bytes < need)) return fail("workspace too small (see dsa_lightning_indexer_bwd_workspace_bytes)");
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return fail("workspace must be 16-byte aligned");
   if (get_status_word(&p.status)) return 1;
-  int err = dsa::launch_indexer_bwd(p, dtype == DSA_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  int err = 0;
+  if (need && dsa::indexer_bwd_dense_fits(p, bf16)) err = dsa::launch_indexer_bwd_dense(p, workspace, &p.only_if, static_cast<cudaStream_t>(stream));
+  if (!err) err = dsa::launch_indexer_bwd(p, bf16, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("lightning_indexer_bwd launch", err) : 0;
 }
 

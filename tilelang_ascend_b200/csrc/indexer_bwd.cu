@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
   float* s_dw = reinterpret_cast<float*>(smem + kOffDw);
   List* lists = reinterpret_cast<List*>(smem + kOffList);
 
+  if (p.only_if && *p.only_if == 0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     *start_status = *reinterpret_cast<volatile int*>(p.status);

@@ -188,10 +188,14 @@ def _indexer_gradients(query, key, weights, indices, d_values):
     d_query, d_weights = torch.empty_like(query), torch.empty_like(weights)
     d_key = torch.zeros(key.shape, dtype=torch.float32, device=dev)
     if B * S1:
+        lib = _lib.load()
+        sizes = B, S1, key.shape[1], N1, D, indices.shape[3], dtype_code(query.dtype)
+        nbytes = lib.dsa_lightning_indexer_bwd_workspace_bytes(*sizes)
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         with on_device(dev):
-            _lib.check(_lib.load().dsa_lightning_indexer_bwd(
+            _lib.check(lib.dsa_lightning_indexer_bwd(
                 query.data_ptr(), key.data_ptr(), weights.data_ptr(), indices.data_ptr(), d_values.data_ptr(), d_query.data_ptr(), d_key.data_ptr(),
-                d_weights.data_ptr(), B, S1, key.shape[1], N1, D, indices.shape[3], dtype_code(query.dtype), raw_stream(dev)))
+                d_weights.data_ptr(), *sizes, ptr(workspace), nbytes, raw_stream(dev)))
     return d_query, d_key, d_weights
 
 
