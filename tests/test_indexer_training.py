@@ -197,10 +197,12 @@ def relative(got, want):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,S1,S2,N1,K", [(1, 1100, 1100, 64, 600), (2, 1030, 1290, 32, 700), (3, 1400, 1061, 16, 1061), (1, 1024, 4000, 64, 2048)])
+@pytest.mark.parametrize("B,S1,S2,N1,K", [(1, 2050, 700, 64, 600), (2, 1030, 1290, 32, 700), (3, 1400, 1061, 16, 1061), (1, 1600, 1600, 64, 1300)])
 def test_gradient_of_lists_that_hold_most_keys(B, S1, S2, N1, K):
     """Long lists of many queries, whose gradients are summed tile by tile: against the definition on the GPU in 64 bits, with holes, keys listed twice,
     queries without keys and padding that was never written."""
+    from tilelang_ascend_b200 import _lib
+    assert _lib.load().dsa_lightning_indexer_bwd_workspace_bytes(B, S1, S2, N1, 128, K, _lib.DTYPE_BF16) > 0   # (that way, then)
     g = torch.Generator().manual_seed(S1 + N1)
     query, key, weights, _ = make_indexer(g, B, S1, S2, N1, 4, torch.bfloat16)
     if S1 <= S2:

@@ -1,4 +1,4 @@
-// Backward of the lightning indexer's listed scores when the lists hold a large part of the keys (sm_100a, tcgen05; bf16, 128 dims, 16,
+// Backward of the lightning indexer's listed scores when the lists hold a large part of the keys that their queries may see (sm_100a, tcgen05; bf16, 128 dims, 16,
 // 32 or 64 heads).  The mathematics is that of indexer_bwd.cu; what differs is how the key gradient is summed.  There every (query, listed key)
 // pair adds 512 bytes to global memory, and those additions are what it takes; here both gradients are products over whole
 // tiles, each owned by the CTA that sums it in tensor memory:
@@ -489,12 +489,20 @@ int launch_both(const IndexerBwdParams& p, const ibd::Dense& d, const CUtensorMa
 }
 }  // namespace
 
-// Lists that hold half of the keys or more (a causal step's then hold three quarters of what its queries may see), and enough
-// queries to fill the chip with tiles.  fp16 stays with the other kernel: its range needs a scale per query.
+// Which kernel: the other one takes about 105 ps per (query, listed key), whatever the heads; these take 60 ps per (query, key that it may
+// see) with 64 heads, half and a quarter of that with 32 and 16, and 20 us more for G and three more launches.  Both counts as they are
+// in a causal step (keys up to S2 - S1 + t) with full lists.  Measured, other / these, us: 4096 queries x 4096 keys, lists of 2048:
+// 671 / 540, of 1024: 410 / 530; 4096 x 8192, 2048: 855 / 1416; 1024 x 4096, 2048: 223 / 278; 4096 x 1024, 512, 16 heads: 258 / 118; 2048 x 2048,
+// 2048, 32 heads: 251 / 121.  fp16 stays with the other kernel: its range needs a scale per query.
 static bool dense_preferred(const IndexerBwdParams& p, bool bf16) {
-  const bool shape = bf16 && p.D == ibd::kD && (p.N1 == 16 || p.N1 == 32 || p.N1 == 64);
-  return shape && static_cast<long long>(p.B) * p.S1 * padded_width(p) <= (1LL << 28) && 2LL * p.K >= p.S2 && static_cast<long long>(p.B) * p.S1 * p.N1 >= 64 * 1024 && p.S2 >= 8 * ibd::kTile &&
-         padded_width(p) / ibd::kTile <= ibd::kMaxSteps && static_cast<long long>(p.B) * p.S1 * p.N1 < (1LL << 30) && static_cast<long long>(p.B) * p.S2 < (1LL << 30);
+  if (!bf16 || p.D != ibd::kD || (p.N1 != 16 && p.N1 != 32 && p.N1 != 64)) return false;
+  const long long B = p.B, S1 = p.S1, S2 = p.S2, K = p.K < p.S2 ? p.K : p.S2;
+  if (B * S1 * padded_width(p) > (1LL << 28) || padded_width(p) / ibd::kTile > ibd::kMaxSteps || B * S1 * p.N1 >= (1LL << 30) || B * S2 >= (1LL << 30)) return false;
+  const long long seen = S1 <= S2 ? S1 * (2 * S2 - S1 + 1) / 2 : S1 * S2;
+  const long long first = S2 - S1 + 1;   // keys that query 0 may see
+  const long long shorter = S1 > S2 || first >= K ? 0 : (K - first < S1 ? K - first : S1);   // queries that see fewer than K
+  const long long listed = S1 * K - (shorter ? shorter * (2 * K - 2 * first - shorter + 1) / 2 : 0);
+  return B * listed * 105 > B * seen * 60 * p.N1 / 64 + 20 * 1000 * 1000;
 }
 
 namespace {
