@@ -163,6 +163,31 @@ def test_strided_and_unaligned_rows(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [70001, 65544])
+def test_wide_rows_in_several_parts(V, dtype):
+    """Rows that several blocks share, in 16-byte units and not, with parts that hold no entry, only masked logits, or the maximum alone."""
+    g, student, teacher, indices = rows(4, V, 900, dtype, "logits", seed=V, listed=True)
+    indices[1] = indices[1] % 3000                    # all entries in the first part (some columns more than once)
+    student[2, 32768:65536] = -INF
+    student[3, V - 1] = 40.0
+    check(student, teacher, indices, "logits", "row", 2.0)
+    check(student, teacher.exp(), indices, "weights", "row", 1.0)
+
+
+@pytest.mark.gpu
+def test_broadcast_rows_and_second_backward():
+    g, student, teacher, indices = rows(5, 600, 40, torch.float32, "weights", seed=12, listed=True)
+    one = student[:1].cuda().requires_grad_()
+    loss = dsa.topk_distillation(one.expand(5, 600), teacher.cuda(), indices.cuda(), over="row")
+    (first,) = torch.autograd.grad(loss.sum(), one, retain_graph=True)
+    (again,) = torch.autograd.grad(loss.sum(), one)
+    _, d, _, slack = definition(student[:1].expand(5, 600), teacher, indices, "weights", "row", 1.0, torch.ones(5))
+    assert torch.equal(first, again)
+    assert bool(((first[0].cpu().double() - d.sum(0)).abs() <= slack.sum(0) + d.abs().sum(0) * 2.0 ** -22).all())
+
+
+@pytest.mark.gpu
 def test_gradient_by_differences():
     g, student, teacher, indices = rows(1, 60, 9, torch.float32, "weights", seed=6, listed=True)
     _, d = check(student, teacher, indices, "weights", "row", 2.0, grad=torch.ones(1))
@@ -214,6 +239,8 @@ def test_refusals():
         lambda: dsa.topk_distillation(s, t, i, over="vocabulary"),
         lambda: dsa.topk_distillation(s, t, i, temperature=0.0),
         lambda: dsa.topk_distillation(s, t, i, temperature=float("inf")),
+        lambda: dsa.topk_distillation(s, t, i, temperature=1e-39),
+        lambda: dsa.topk_distillation(s, t, i, temperature=float("nan")),
         lambda: dsa.topk_distillation(s[:, ::2], t, i),
         lambda: dsa.topk_distillation(torch.zeros(10, 4).t(), t, i),
         lambda: dsa.topk_distillation(s, torch.ones(3, 4).t(), i),

@@ -409,6 +409,91 @@ def test_captured_and_on_another_stream():
     check_status()
 
 
+@pytest.mark.gpu
+def test_calls_at_the_same_time_and_two_graphs():
+    """Calls that overlap on two streams, and two graphs of one call replayed in turn, do not touch one another's results: sizes that take each of the two
+    ways through the indexer's backward."""
+    g = torch.Generator().manual_seed(15)
+    small = [t.cuda() for t in make_indexer(g, 2, 60, 500, 64, 200, torch.bfloat16)]
+    large = [t.cuda() for t in make_indexer(g, 1, 1500, 1500, 16, 1400, torch.bfloat16)]
+    grads = [torch.randn(s[3].shape, generator=g).cuda() for s in (small, large)]
+    q, kv = torch.randn((1, 300, 128, 576), generator=g).to(torch.bfloat16).cuda(), torch.randn((1, 700, 1, 576), generator=g).to(torch.bfloat16).cuda()
+    idx, lse = lists(g, 1, 300, 700, 300).cuda(), torch.randn((1, 300, 128), generator=g).cuda() + 6
+
+    def step(which):
+        dq, dk, dw = dsa.lightning_indexer_bwd_raw(*(small, large)[which], grads[which])
+        return dq, dw, dsa.sparse_mla_key_weights(q, kv, idx, lse)
+
+    want = [step(0), step(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, captured = [], []
+    for i, stream in enumerate(streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                captured.append(step(i))
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = [None, None]
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = step(i)
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])) and all(torch.equal(a, b) for a, b in zip(captured[i], want[i]))
+    check_status()
+
+
+@pytest.mark.gpu
+def test_a_whole_step_in_a_graph():
+    """Forward and backward of the distillation through autograd, captured and replayed on other inputs."""
+    g = torch.Generator().manual_seed(16)
+    query, key, weights, _ = make_indexer(g, 1, 1500, 1500, 16, 4, torch.bfloat16)
+    leaves = [t.cuda().requires_grad_() for t in (query, key, weights)]
+    indices, values = dsa.lightning_indexer_raw(*[t.detach() for t in leaves], sparse_count=1400, sparse_mode=3, return_value=True)
+    teacher = torch.rand(indices.shape, generator=g).cuda()
+
+    def step():
+        loss = dsa.lightning_indexer_distillation(*leaves, indices, values, teacher)
+        return (loss.detach(),) + torch.autograd.grad(loss.sum(), leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured = step()
+    torch.cuda.synchronize()
+    teacher.copy_(torch.rand(indices.shape, generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    again = step()
+    assert all(torch.equal(captured[i], again[i]) for i in (0, 1, 3)) and relative(captured[2], again[2].cpu().double()) < 2.0 ** -7
+    check_status()
+
+
+@pytest.mark.gpu
+def test_weights_of_any_alignment_and_other_head_counts():
+    """Head weights off a 16-byte boundary, and 48 heads, where the lists hold most keys."""
+    g = torch.Generator().manual_seed(17)
+    for N1, offset in ((32, 1), (48, 0)):
+        query, key, weights, indices = (t.cuda() for t in make_indexer(g, 2, 1030, 1290, N1, 700, torch.bfloat16))
+        buffer = torch.zeros(weights.numel() + 4, device="cuda")
+        moved = buffer[offset:offset + weights.numel()].view(weights.shape)
+        moved.copy_(weights)
+        d_values = torch.randn(indices.shape, generator=g).cuda()
+        dq, dk, dw = dsa.lightning_indexer_bwd_raw(query, key, moved, indices, d_values)
+        # the same through fp16, whose gradient always takes the other way (values of eight bits are exact in both types)
+        hq, hk, hw = dsa.lightning_indexer_bwd_raw(query.half(), key.half(), weights, indices, d_values)
+        for got, ref, bound in ((dq, hq, 2 * 2.0 ** -8), (dk, hk, 2 * 2.0 ** -8), (dw, hw, 2.0 ** -18)):
+            assert relative(got, ref.cpu().double()) <= bound
+    check_status()
+
+
 # --------------------------------------------------------------------------------------------------------- refusals
 def test_refusals():
     q, kv = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16), torch.zeros(1, 9, 1, 64, dtype=torch.bfloat16)

@@ -224,6 +224,28 @@ def test_cached_rows_go_to_their_slots_and_no_others(parts, D, start, slot_dtype
 
 
 @pytest.mark.gpu
+def test_a_bias_without_a_weight_and_rows_used_twice():
+    g, q, _, positions, inv_freq = make(2, 4, 3, 1, 128, 64, torch.bfloat16, seed=21)
+    bias = (0.3 * torch.randn(128, generator=g)).float()
+    leaf, b = q.cuda().requires_grad_(), bias.cuda().requires_grad_()
+    oq, ok = dsa.qk_norm_rope(leaf, leaf, positions.cuda(), inv_freq.cuda(), q_norm="layer", q_bias=b)
+    (oq.float().sum() * 2 + ok.float().sum()).backward()
+    x, bd = q.double().requires_grad_(), bias.double().requires_grad_()
+    ref = reference(x, positions, inv_freq, "layer", None, bd, 128, 0, True, 1.0, 1e-6)
+    assert_rounded(oq, ref.detach(), ROW * 3 * ref.detach().abs().amax(-1, keepdim=True), "q'")
+    two = reference(x, positions, inv_freq, None, None, None, 128, 0, True, 1.0, 1e-6)
+    dx, db = torch.autograd.grad(ref.sum() * 2 + two.sum(), (x, bd))
+    # two gradients of the leaf, each rounded, and their sum: 3 half steps of the two parts (each at most 3, the norm's terms cancel)
+    assert float((leaf.grad.cpu().double() - dx).abs().max()) <= 3 * 2.0 ** -8 * 6
+    assert_rounded(b.grad, db, 1e-4, "dbias")
+    # a side whose output is not used asks for nothing
+    leaf2, k2 = q.cuda().requires_grad_(), q.cuda().requires_grad_()
+    oq, ok = dsa.qk_norm_rope(leaf2, k2, positions.cuda(), inv_freq.cuda(), q_norm="rms", k_norm="rms")
+    ok.sum().backward()
+    assert leaf2.grad is None and k2.grad is not None
+
+
+@pytest.mark.gpu
 def test_masked_values_and_empty_calls():
     """Infinities and NaN stay in their own row; calls without tokens return empty tensors; the sums of no rows are zeros."""
     _, q, k, positions, inv_freq = make(1, 6, 3, 1, 128, 64, torch.bfloat16, seed=8)

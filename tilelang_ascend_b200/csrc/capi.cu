@@ -149,7 +149,8 @@ int fill_distill(dsa::DistillParams* p, const void* student, int32_t student_dty
   if (student_dtype < 0 || student_dtype > 2 || teacher_dtype < 0 || teacher_dtype > 2) return fail("dtypes must be 0 (bfloat16), 1 (float16) or 2 (float32)");
   if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || K <= 0 || V > 0x7fffffff - 65536) return fail("rows, V and K must be positive (rows and V below 2^31)");
   if (!indices && K != V) return fail("without indices K must equal V");
-  if (!(temperature > 0.f) || !std::isfinite(temperature)) return fail("temperature must be positive and finite");
+  if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(static_cast<float>(1.4426950408889634 / temperature)))
+    return fail("temperature must be positive and finite, and so must its reciprocal");
   if (reinterpret_cast<uintptr_t>(stats) & 15u) return fail("stats must be 16-byte aligned");
   *p = dsa::DistillParams{};
   p->student = student; p->teacher = teacher; p->indices = indices; p->stats = const_cast<float*>(stats);

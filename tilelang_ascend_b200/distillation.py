@@ -26,8 +26,8 @@ def _check_rows(student, teacher, indices, teacher_kind, over, temperature) -> t
         raise ValueError(f"teacher_kind must be 'weights' or 'logits', got {teacher_kind!r}")
     if over not in _OVER:
         raise ValueError(f"over must be 'list' or 'row', got {over!r}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be in [1e-30, 1e30], got {temperature}")
     for t, name in ((student, "student"), (teacher, "teacher")):
         if not isinstance(t, torch.Tensor) or t.dim() < 1:
             raise ValueError(f"{name} must be a tensor of rows")
