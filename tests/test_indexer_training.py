@@ -246,6 +246,32 @@ def test_gradient_of_lists_that_hold_most_keys(B, S1, S2, N1, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["query", "key", "weights"])
+def test_unlisted_values_whose_products_overflow(where):
+    """Finite, but with infinite products: rows that take part in no listed pair leave the gradients as they are."""
+    g = torch.Generator().manual_seed(29)
+    B, S1, S2, N1, K = 1, 1501, 1280, 32, 1279
+    query, key, weights, _ = (t.cuda() for t in make_indexer(g, B, S1, S2, N1, 4, torch.bfloat16))
+    indices = torch.arange(K, dtype=torch.int32).expand(B, S1, 1, K).clone()   # not key 1279
+    indices[0, 40] = -1
+    indices = indices.cuda()
+    d_values = torch.randn(indices.shape, generator=g).cuda() * 1e-3
+    want = dsa.lightning_indexer_bwd_raw(query, key, weights, indices, d_values)
+    if where == "query":
+        query[0, 40] = 3e38
+    elif where == "key":
+        key[0, S2 - 1] = -3e38
+    else:
+        weights[0, 40] = 3e38
+    got = dsa.lightning_indexer_bwd_raw(query, key, weights, indices, d_values)
+    # (two kernels' gradients: each within the bounds of the test above)
+    for name, a, b, bound in zip("qkw", got, want, (4 * 2.0 ** -8, 2 * 2.0 ** -8, 2 * 2.0 ** -18)):
+        assert bool(torch.isfinite(a.float()).all()) and relative(a, b.cpu().double()) <= bound, f"d{name}"
+    assert not got[0][0, 40].any() and not got[2][0, 40].any() and not got[1][0, S2 - 1].any()
+    check_status()
+
+
+@pytest.mark.gpu
 def test_a_key_listed_twice_counts_twice():
     g = torch.Generator().manual_seed(11)
     query, key, weights, indices = make_indexer(g, 1, 3, 200, 64, 64, torch.bfloat16)

@@ -4,15 +4,21 @@
 // tiles, each owned by the CTA that sums it in tensor memory:
 //
 //   spread   the lists' gradients become a matrix G [B, S1, S2 padded to 128] (0 where not listed) and a flag per (query, tile of 128 keys)
-//   kQueries a CTA owns 128 (query, head) rows and walks the key tiles:    dQ^T[128 dims x 128 rows] += K^T dZ,  and dw
-//   kKeys    a CTA owns 128 keys and walks blocks of 128 (query, head) rows:  dK^T[128 dims x 128 keys] += Q^T dZ^T
+//   kQueries a CTA owns 128 (query, head) rows and walks the key tiles:              dQ[128 rows x 128 dims] += dZ K,  and dw
+//   kKeys    a CTA owns 128 keys and walks blocks of 128 (query, head) rows:         dK[128 keys x 128 dims] += dZ Q
 //
-// with Z[128 keys x 128 rows] = K Q^T and dZ = G w [Z > 0] made once in each.  Tiles are dense, so they come by TMA, without
-// indices; (block, tile) pairs without a listed key are skipped by the flags (the upper half of a causal step).  1024 clocks of MMAs
-// per pair of tiles and kernel.
-// A dense product also multiplies what is not listed, by 0.  Where that holds infinities or NaN (padding that was never written), 0
-// is the wrong answer, so `spread` looks through q and k for them; if there are any, these kernels do nothing and the other kernel,
-// launched behind them, does it all.
+// with Z[128 own x 128 walked] = own . walked and dZ = G w [Z > 0], made once in each.  The walked tile is read twice from shared memory,
+// K-major for Z and MN-major for the sum; dZ goes to tensor memory, over the columns of Z that have been read, so that the sum takes its
+// first operand there.  What bounds a step is the way from Z to dZ to the sum's MMAs (about 3900 clocks, of which the two
+// products are 1024), so three steps are under way: three places for Z, each with four warps that turn Z into dZ all by themselves
+// (no barrier among them), and the group that has an item's last step reads the sum out while the others go on.  Measured for 4096 queries x 2048
+// of 4096 keys, 64 heads: kQueries 214 and kKeys 224 us (310 TFLOP/s of listed pairs each); with dZ in shared memory and all 16 warps at one
+// step 257 and 244, of which the MMAs and the loads were not the bound (left out, the time stayed), the warps' 3200 clocks for two steps were.
+// Tiles are dense, so they come by TMA, without indices; (block, tile) pairs without a listed key are skipped by the flags (the upper
+// half of a causal step).
+// A dense product also multiplies what is not listed, by 0.  Where that holds infinities, NaN or values whose products overflow
+// (padding that was never written), 0 is the wrong answer, so `spread` looks through q, k and w for them; if there are any, these
+// kernels do nothing and the other kernel, launched behind them, does it all.
 #include <stdint.h>
 #include <string.h>
 
@@ -25,37 +31,25 @@ namespace dsa {
 
 namespace ibd {
 constexpr int kD = 128, kTile = 128;                                  // dims; keys or (query, head) rows of a tile
-constexpr uint32_t kChunk = kTile * 128, kTileBytes = 2 * kChunk;     // two chunks of 64 dims (dZ: of 64 rows)
-constexpr int kStages = 3;
+constexpr uint32_t kChunk = kTile * 128, kTileBytes = 2 * kChunk;     // two chunks of 64 dims
+constexpr uint32_t kSideBytes = 4096;                                 // beside a walked tile: its gradients (kQueries: up to eight queries' 128 keys) or head weights
+constexpr int kStages = 4, kSlots = 3;                                // walked tiles in shared memory; Z and dZ in tensor memory
 constexpr int kMaxSteps = 1024;                                       // tiles an item may walk
-constexpr int kWorkers = 16, kLoadWarp = 16, kZWarp = 17, kMmaWarp = 18, kListWarp = 19, kThreads = 20 * 32;
+constexpr int kWorkers = 4 * kSlots, kLoadWarp = kWorkers, kZWarp = kWorkers + 1, kMmaWarp = kWorkers + 2, kListWarp = kWorkers + 3, kThreads = (kWorkers + 4) * 32;
 constexpr int kUsers = kWorkers + 3;
 struct Steps {
   int item, count;               // item -1: no more
   int pad[2];
   uint16_t step[kMaxSteps];
 };
-constexpr uint32_t kOffRing = kTileBytes, kOffDz = kOffRing + kStages * kTileBytes;
-constexpr uint32_t kOffBar = kOffDz + 2 * kTileBytes;
-constexpr uint32_t kOffW = kOffBar + 256;                             // head weights of the stages' rows, and of the own ones
-constexpr uint32_t kOffDw = kOffW + (kStages + 1) * kTile * 4;        // four quarters' sums of 128 rows
-constexpr uint32_t kOffSteps = kOffDw + 4 * kTile * 4;
+constexpr int kDwItems = 3;
+constexpr uint32_t kOffRing = 2 * kTileBytes, kOffSide = kOffRing + kStages * kTileBytes;   // (two own tiles first)
+constexpr uint32_t kOffBar = kOffSide + kStages * kSideBytes;
+constexpr uint32_t kOffDw = kOffBar + 256;                            // sums of 128 rows by the groups, of three items
+constexpr uint32_t kOffSteps = kOffDw + kDwItems * kSlots * kTile * 4;
 constexpr uint32_t kSmemBytes = kOffSteps + 2 * sizeof(Steps);
-constexpr uint32_t kColZ = 0, kColAcc = 256, kTmemCols = 512;         // two of each, 128 columns
+constexpr uint32_t kColZ = 0, kColAcc = kSlots * kTile, kTmemCols = 512;      // three of Z (dZ takes the first 64 columns of its own), the sum
 static_assert(kSmemBytes <= 232448, "shared memory per CTA");
-
-__device__ __forceinline__ bool bar_and(uint32_t id, uint32_t nthreads, bool yes) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(yes ? 1u : 0u), "r"(id), "r"(nthreads)
-      : "memory");
-  return all != 0;
-}
 
 // Contiguous global -> shared copy (16-byte aligned addresses, size a multiple of 16); its bytes count on the barrier.
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t mbar) {
@@ -63,25 +57,31 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
                : "memory");
 }
 
+// Adds four fp32 values (given as bits) to 16-byte aligned global memory.
+__device__ __forceinline__ void red_add_v4(float* dst, uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(__uint_as_float(a)), "f"(__uint_as_float(b)),
+               "f"(__uint_as_float(c)), "f"(__uint_as_float(e))
+               : "memory");
+}
+
 struct Dense {
-  const int* dirty;       // not 0: q or k hold infinities or NaN, nothing is done
+  const int* dirty;       // not 0: q, k or w hold what must not be multiplied by 0; nothing is done
   int* next;              // [2] items handed out so far
   const float* grad;      // G [B, S1, width]
   const uint8_t* flags;   // [B, S1, width / 128]
   int width, tiles;       // S2 rounded up to 128; width / 128
-  int queries;            // per block of 128 rows
   int blocks;             // of a batch entry's queries
   int splits, per_split;  // kKeys: parts a key tile's blocks are walked in
 };
 }  // namespace ibd
 
 // -------------------------------------------------------------------------------------------------
-// spread: block = (query, 8192 columns of G).  The blocks also look through q (each its query) and k (each its share of the rows).
+// spread: block = (query, 8192 columns of G).  The blocks also look through q and w (each its query) and k (each its share of the rows).
 // -------------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
     indexer_bwd_spread_kernel(const __grid_constant__ IndexerBwdParams p, float* G, uint8_t* flags, int* dirty, const int width, const int parts, const int k_units) {
-  // bf16 infinities and NaN: all bits of the exponent
-  auto odd_pair = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+  // bf16 infinities, NaN and values from 2^60 on (128 products of smaller ones stay finite)
+  auto odd_pair = [](uint32_t w) { return (w & 0x7f80u) >= 0x5d80u || (w & 0x7f800000u) >= 0x5d800000u; };
   auto odd = [&](const uint4& v) { return odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w); };
   constexpr int kCols = 8192;
   __shared__ __align__(16) float acc[kCols];
@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(256)
     const uint4* q = reinterpret_cast<const uint4*>(p.q) + bt * p.N1 * 16;
 #pragma unroll 4
     for (int i = tid; i < p.N1 * 16; i += 256) found |= odd(__ldg(q + i));
+    if (tid < p.N1) found |= !(fabsf(__ldg(p.w + bt * p.N1 + tid)) < 0x1p60f);
     const uint4* k = reinterpret_cast<const uint4*>(p.k);
     const int64_t last = min(static_cast<int64_t>(p.B) * p.S2 * 16, (bt + 1) * k_units);
     for (int64_t i = bt * k_units + tid; i < last; i += 256) found |= odd(__ldg(k + i));
@@ -137,29 +138,27 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
     indexer_bwd_dense_kernel(const __grid_constant__ IndexerBwdParams p, const __grid_constant__ ibd::Dense d, const __grid_constant__ CUtensorMap q_map,
                              const __grid_constant__ CUtensorMap k_map) {
   using namespace ibd;
-  constexpr int kCols = 32, kMine = N1 < kCols ? kCols / N1 : 1;   // a worker's columns; queries among them when they are rows
+  constexpr int kMine = kTile / N1;   // queries of a block of rows
   extern __shared__ __align__(1024) uint8_t smem[];
-  const uint32_t sOwn = smem_u32(smem);
+  const uint32_t sOwn = smem_u32(smem), sRing = sOwn + kOffRing, sSide = sOwn + kOffSide;
   if (sOwn & 1023u) {
     if (threadIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusBadLayout);
     return;
   }
-  const uint32_t sRing = sOwn + kOffRing, sDz = sOwn + kOffDz;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint64_t* own_full = bars;         // count 1 + transaction bytes: the item's own tile has landed
-  uint64_t* own_done = bars + 1;     // count 1: commit after an item's last MMAs: its own tile is free, its sum is complete
-  uint64_t* full = bars + 2;         // [3] count 1 + transaction bytes
-  uint64_t* empty = bars + 5;        // [3] count 1: commit after the MMAs that read the stage
-  uint64_t* z_full = bars + 8;       // [2] count 1: commit after Z
-  uint64_t* z_free = bars + 10;      // [2] count 16: Z has been read
-  uint64_t* dz_full = bars + 12;     // [2] count 16: dZ is in shared memory
-  uint64_t* dz_free = bars + 14;     // [2] count 1: commit after the MMAs that read dZ
-  uint64_t* acc_free = bars + 16;    // [2] count 16: the sum has been read
-  uint64_t* list_full = bars + 18;   // [2] count 1
-  uint64_t* list_free = bars + 20;   // [2] count kUsers
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
-  int* start_status = reinterpret_cast<int*>(bars + 23);
-  float* s_w = reinterpret_cast<float*>(smem + kOffW);
+  uint64_t* full = bars;             // [4] count 1 + transaction bytes
+  uint64_t* empty = bars + 4;        // [4] count 1: commit after the MMAs that read the stage
+  uint64_t* own_full = bars + 8;     // [2] count 1 + transaction bytes
+  uint64_t* own_free = bars + 10;    // [2] count 1: commit after an item's last Z
+  uint64_t* dw_full = bars + 12;     // count kWorkers: an item's dw by group
+  uint64_t* acc_free = bars + 13;    // count 4: the sum has been read
+  uint64_t* z_full = bars + 14;      // [3] count 1: commit after Z
+  uint64_t* dz_full = bars + 17;     // [3] count 4: dZ is in tensor memory
+  uint64_t* dz_free = bars + 20;     // [3] count 1: commit after the MMAs that read dZ
+  uint64_t* list_full = bars + 23;   // [2] count 1
+  uint64_t* list_free = bars + 25;   // [2] count kUsers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
+  int* start_status = reinterpret_cast<int*>(bars + 28);
   float* s_dw = reinterpret_cast<float*>(smem + kOffDw);
   Steps* lists = reinterpret_cast<Steps*>(smem + kOffSteps);
 
@@ -167,13 +166,19 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
   if (*d.dirty) return;
   if (tid == 0) {
     *start_status = *reinterpret_cast<volatile int*>(p.status);
-    mbar_init(own_full, 1); mbar_init(own_done, 1);
     for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(&z_full[i], 1); mbar_init(&dz_full[i], 4); mbar_init(&dz_free[i], 1); }
+    mbar_init(dw_full, kWorkers); mbar_init(acc_free, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&z_full[i], 1); mbar_init(&z_free[i], kWorkers); mbar_init(&dz_full[i], kWorkers); mbar_init(&dz_free[i], 1);
-      mbar_init(&acc_free[i], kWorkers); mbar_init(&list_full[i], 1); mbar_init(&list_free[i], kUsers);
+      mbar_init(&own_full[i], 1); mbar_init(&own_free[i], 1);
+      mbar_init(&list_full[i], 1); mbar_init(&list_free[i], kUsers);
     }
     mbar_init_fence();
+  }
+  if constexpr (kOwner == kKeys) {
+    // a block's rows may end before its tile: what the stage held before is multiplied by 0, so it has to be finite
+    for (int i = tid; i < kStages * kTile; i += kThreads) reinterpret_cast<float*>(smem + kOffSide + i / kTile * kSideBytes)[i % kTile] = 0.f;
+    fence_proxy_async_smem();
   }
   if (warp == kMmaWarp) { tmem_alloc(tmem_slot, kTmemCols); tmem_relinquish(); }
   tc_fence_before();
@@ -182,13 +187,18 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   bool ok = *start_status == kStatusOk;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
-  // two at once: the answer of a barrier takes 200 clocks and more on this busy shared memory
+  // two at once: the answer of a barrier takes 200 clocks and more on a busy shared memory
   auto wait_both = [&](uint64_t* a, uint32_t parity_a, uint64_t* b, uint32_t parity_b, bool b_needed) {
     const bool got_a = mbar_try_wait(a, parity_a), got_b = !b_needed || mbar_try_wait(b, parity_b);
     return __all_sync(0xffffffffu, got_a && got_b) || (wait(a, parity_a) && (!b_needed || wait(b, parity_b)));
   };
   auto use = [](int n) { return static_cast<uint32_t>(n >> 1) & 1u; };           // parity of the n-th use of one of two
   auto before = [](int n) { return (static_cast<uint32_t>(n >> 1) + 1u) & 1u; }; // of the use before it
+  // step g of all items: its stage and its slot, and the parity of their use number g / count (the one before it: ^ 1)
+  auto stage_of = [](int g) { return g % kStages; };
+  auto lap = [](int g) { return static_cast<uint32_t>(g / kStages) & 1u; };
+  auto slot_of = [](int g) { return g % kSlots; };
+  auto turn = [](int g) { return static_cast<uint32_t>(g / kSlots) & 1u; };
   auto done_with = [&](int n) {
     __syncwarp();
     if (lane == 0) mbar_arrive(&list_free[n & 1]);
@@ -217,20 +227,19 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
       int count = 0;
       for (int s0 = first; s0 < last; s0 += 32) {
         const int s = s0 + lane, tile = kOwner == kQueries ? s : own, block = kOwner == kQueries ? own : s;
-        bool any = false;
-        if (s < last)
-          for (int k = 0; k < d.queries; ++k) {
-            const int query = block * d.queries + k;
-            any |= query < p.S1 && __ldg(flags + static_cast<int64_t>(query) * d.tiles + tile) != 0;
-          }
-        const uint32_t bits = __ballot_sync(0xffffffffu, any);
+        uint32_t any = 0;
+        if (s < last) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) any |= __ldg(flags + static_cast<int64_t>(min(block * kMine + k, p.S1 - 1)) * d.tiles + tile);
+        }
+        const uint32_t bits = __ballot_sync(0xffffffffu, any != 0);
         if (any) list.step[count + __popc(bits & ((1u << lane) - 1))] = static_cast<uint16_t>(s);
         count += __popc(bits);
       }
       if (!count) {
         if (kOwner == kQueries) {   // rows without a key: zeros
-          const int rows = min(kTile, (p.S1 - own * d.queries) * N1);
-          const int64_t row0 = (static_cast<int64_t>(b) * p.S1 + own * d.queries) * N1;
+          const int rows = min(kTile, (p.S1 - own * kMine) * N1);
+          const int64_t row0 = (static_cast<int64_t>(b) * p.S1 + own * kMine) * N1;
           uint4* dq = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.d_q) + row0 * kD);
           for (int k = lane; k < rows * kD / 8; k += 32) dq[k] = make_uint4(0, 0, 0, 0);
           for (int k = lane; k < rows; k += 32) p.d_w[row0 + k] = 0.f;
@@ -256,38 +265,48 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
     const CUtensorMap* own_map = kOwner == kQueries ? &q_map : &k_map;
     const CUtensorMap* walk_map = kOwner == kQueries ? &k_map : &q_map;
     if (lane == 0) { prefetch_tensormap(own_map); prefetch_tensormap(walk_map); }
-    int g = 0;
-    for (int n = 0; ok; ++n) {
+    int g = 0, n = 0;   // steps and own tiles asked for
+    while (ok) {
       if (!wait(&list_full[n & 1], use(n))) { ok = false; break; }
       const Steps& list = lists[n & 1];
       const int item = list.item;
       if (item < 0) break;
-      const int b = batch_of(item), own = owned(item);
-      const int q_row0 = b * p.S1 * N1, k_row0 = b * p.S2;
-      if (n >= 1 && !wait(own_done, (n + 1) & 1)) { ok = false; break; }
-      // the head weights of a block of rows travel with them
-      auto weight_bytes = [&](int block) { return static_cast<uint32_t>(min(kTile, p.S1 * N1 - block * kTile)) * 4u; };
-      const float* weights = p.w + static_cast<int64_t>(q_row0);
+      const int b = batch_of(item), own = owned(item), count = list.count;
+      const int q_row0 = b * p.S1 * N1, k_row0 = b * p.S2, own_row0 = kOwner == kQueries ? q_row0 : k_row0, walk_row0 = kOwner == kQueries ? k_row0 : q_row0;
+      const int own_queries = min(kMine, p.S1 - own * kMine);   // (kQueries)
+      if (n >= 2 && !wait(&own_free[n & 1], before(n))) { ok = false; break; }
       if (lane == 0) {
-        mbar_arrive_expect_tx(own_full, kTileBytes + (kOwner == kQueries ? weight_bytes(own) : 0u));
-        if (kOwner == kQueries) bulk_load(smem_u32(s_w + kStages * kTile), weights + own * kTile, weight_bytes(own), smem_u32(own_full));
-        for (int c = 0; c < 2; ++c) tma_load_2d(sOwn + c * kChunk, own_map, smem_u32(own_full), c * 64, (kOwner == kQueries ? q_row0 : k_row0) + own * kTile);
+        mbar_arrive_expect_tx(&own_full[n & 1], kTileBytes);
+        for (int c = 0; c < 2; ++c)
+          tma_load_2d(sOwn + (n & 1) * kTileBytes + c * kChunk, own_map, smem_u32(&own_full[n & 1]), c * 64, own_row0 + own * kTile);
       }
       __syncwarp();
-      for (int i = 0; i < list.count; ++i, ++g) {
-        const int s = g % kStages;
-        if (g >= kStages && !wait(&empty[s], ((g / kStages) + 1) & 1)) { ok = false; break; }
+      for (int i = 0; i < count; ++i, ++g) {
+        const int s = stage_of(g);
+        if (g >= kStages && !wait(&empty[s], lap(g) ^ 1u)) { ok = false; break; }
         if (lane == 0) {
-          mbar_arrive_expect_tx(&full[s], kTileBytes + (kOwner == kKeys ? weight_bytes(list.step[i]) : 0u));
-          if (kOwner == kKeys) bulk_load(smem_u32(s_w + s * kTile), weights + list.step[i] * kTile, weight_bytes(list.step[i]), smem_u32(&full[s]));
-          for (int c = 0; c < 2; ++c)
-            tma_load_2d(sRing + s * kTileBytes + c * kChunk, walk_map, smem_u32(&full[s]), c * 64, (kOwner == kQueries ? k_row0 : q_row0) + list.step[i] * kTile);
+          const int tile = list.step[i];
+          const uint32_t bar = smem_u32(&full[s]), side = sSide + s * kSideBytes;
+          // beside a key tile the gradients of the own block's queries, beside a block of rows their head weights
+          const uint32_t side_bytes = kOwner == kQueries ? static_cast<uint32_t>(own_queries) * kTile * 4u : static_cast<uint32_t>(min(kTile, p.S1 * N1 - tile * kTile)) * 4u;
+          mbar_arrive_expect_tx(&full[s], kTileBytes + side_bytes);
+          for (int c = 0; c < 2; ++c) tma_load_2d(sRing + s * kTileBytes + c * kChunk, walk_map, bar, c * 64, walk_row0 + tile * kTile);
+          if constexpr (kOwner == kQueries) {
+            for (int k = 0; k < own_queries; ++k)
+              bulk_load(side + k * kTile * 4, d.grad + (static_cast<int64_t>(b) * p.S1 + own * kMine + k) * d.width + tile * kTile, kTile * 4, bar);
+          } else {
+            bulk_load(side, p.w + static_cast<int64_t>(q_row0) + tile * kTile, side_bytes, bar);
+          }
         }
         __syncwarp();
       }
-      if (!ok) break;
-      done_with(n);
+      if (!ok) { ++n; break; }
+      done_with(n++);
     }
+    // given up: the copies in flight land before the shared memory goes
+    auto landed = [&](uint64_t* bar, uint32_t parity) { for (int tries = 0; tries < (1 << 16) && !mbar_try_wait(bar, parity); ++tries) {} };
+    for (int i = max(g - kStages, 0); !ok && i < g; ++i) landed(&full[stage_of(i)], lap(i));
+    for (int i = max(n - 2, 0); !ok && i < n; ++i) landed(&own_full[i & 1], use(i));
   } else if (warp == kZWarp) {
     // ================================ MMA issuer of Z (converged, one elected lane issues) ==========
     constexpr uint32_t idesc = make_idesc_f16(true, kTile, kTile, 0, 0);
@@ -297,169 +316,182 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
       if (!wait(&list_full[n & 1], use(n))) { ok = false; break; }
       const int count = __reduce_or_sync(0xffffffffu, lists[n & 1].item < 0 ? 0u : static_cast<uint32_t>(lists[n & 1].count));
       if (!count) break;
-      if (!wait(own_full, n & 1)) { ok = false; break; }
+      if (!wait(&own_full[n & 1], use(n))) { ok = false; break; }
+      const uint64_t da = make_smem_desc(sOwn + (n & 1) * kTileBytes, 16, 1024, kSwizzle128B);
       for (int i = 0; i < count; ++i, ++g) {
-        const int s = g % kStages;
-        if (!wait_both(&full[s], (g / kStages) & 1, &z_free[g & 1], before(g), g >= 2)) { ok = false; break; }
+        const int s = stage_of(g), slot = slot_of(g);
+        if (!wait_both(&full[s], lap(g), &dz_free[slot], turn(g) ^ 1u, g >= kSlots)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t walked = sRing + s * kTileBytes, keys = kOwner == kQueries ? walked : sOwn, rows = kOwner == kQueries ? sOwn : walked;
+        const uint64_t db = make_smem_desc(sRing + s * kTileBytes, 16, 1024, kSwizzle128B);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint64_t da = make_smem_desc(keys + c * kChunk, 16, 1024, kSwizzle128B), db = make_smem_desc(rows + c * kChunk, 16, 1024, kSwizzle128B);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_ss_if(go, tmem + kColZ + (g & 1) * kTile, da + 2 * k, db + 2 * k, idesc, (c | k) != 0);
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t at = (k >> 2) * (kChunk >> 4) + 2 * (k & 3);
+          umma_ss_if(go, tmem + kColZ + slot * kTile, da + at, db + at, idesc, k != 0);
         }
-        umma_commit_if(go, &z_full[g & 1]);
+        umma_commit_if(go, &z_full[slot]);
       }
       if (!ok) break;
+      umma_commit_if(go, &own_free[n & 1]);
       done_with(n);
     }
   } else if (warp == kMmaWarp) {
     // ================================ MMA issuer of the sums ========================================
-    constexpr uint32_t idesc = make_idesc_f16(true, kD, kTile, 1, kOwner == kQueries ? 1 : 0);
+    constexpr uint32_t idesc = make_idesc_f16(true, kTile, kD, 0, 1);
     const uint32_t go = elect_one_lane(), tmem = __reduce_or_sync(0xffffffffu, tmem_base);
     int g = 0;
     for (int n = 0; ok; ++n) {
       if (!wait(&list_full[n & 1], use(n))) { ok = false; break; }
       const int count = __reduce_or_sync(0xffffffffu, lists[n & 1].item < 0 ? 0u : static_cast<uint32_t>(lists[n & 1].count));
       if (!count) break;
-      if (n >= 2 && !wait(&acc_free[n & 1], before(n))) { ok = false; break; }
+      if (n >= 1 && !wait(acc_free, (n + 1) & 1)) { ok = false; break; }
       for (int i = 0; i < count; ++i, ++g) {
-        const int s = g % kStages;
-        if (!wait(&dz_full[g & 1], use(g))) { ok = false; break; }
-        fence_proxy_async_smem();
+        const int s = stage_of(g), slot = slot_of(g);
+        if (!wait(&dz_full[slot], turn(g))) { ok = false; break; }
         tc_fence_after();
-        // A: the walked tile read MN-major (128 dims; contraction over its keys or rows); B: dZ, rows are keys, two chunks of 64 (query, head) rows:
-        // MN-major over the keys (kQueries), K-major over the rows (kKeys)
-        const uint32_t dz = sDz + (g & 1) * kTileBytes;
-        const uint64_t da = make_smem_desc(sRing + s * kTileBytes, kChunk, 1024, kSwizzle128B);
-        const uint64_t db = kOwner == kQueries ? make_smem_desc(dz, kChunk, 1024, kSwizzle128B) : make_smem_desc(dz, 16, 1024, kSwizzle128B);
+        const uint64_t db = make_smem_desc(sRing + s * kTileBytes, kChunk, 1024, kSwizzle128B);   // the walked tile read MN-major: 128 dims, contraction over its rows
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t step = kOwner == kQueries ? k * (2048 >> 4) : ((k >> 2) * (kChunk >> 4) + 2 * (k & 3));
-          umma_ss_if(go, tmem + kColAcc + (n & 1) * kTile, da + k * (2048 >> 4), db + step, idesc, (i | k) != 0);
-        }
+        for (int k = 0; k < 8; ++k)
+          umma_ts_if(go, tmem + kColAcc, tmem + kColZ + slot * kTile + k * 8, db + k * (2048 >> 4), idesc, (i | k) != 0);
         umma_commit_if(go, &empty[s]);
-        umma_commit_if(go, &dz_free[g & 1]);
+        umma_commit_if(go, &dz_free[slot]);
       }
       if (!ok) break;
-      umma_commit_if(go, own_done);
       done_with(n);
     }
   } else {
     // ================================ dZ and dw; the sums to global memory ==========================
-    // warp = (quarter, group): key 32 quarter + lane and rows 32 group .. + 31 of Z; dim 32 quarter + lane and columns 32 group .. + 31 of a sum
-    const int quarter = warp & 3, group = warp >> 2, key = quarter * 32 + lane;
+    // Group = four warps = the steps of one slot; warp = a quarter of its lanes: own row or key 32 quarter + lane, all 128 walked columns.
+    const int quarter = warp & 3, group = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     int g = 0;
-    // (Every warp of the group takes the same turns, also when a wait has given up: the barriers count them all.)
-    for (int n = 0;; ++n) {
-      ok = bar_and(1, kWorkers * 32, ok && wait(&list_full[n & 1], use(n)));
-      if (!ok) break;
+    // The group of an item's last step reads the sums, while the others go on to the next item; it has its turn there last.
+    for (int n = 0; ok; ++n) {
+      if (!wait(&list_full[n & 1], use(n))) { ok = false; break; }
       const Steps& list = lists[n & 1];
       const int item = list.item;
       if (item < 0) break;
       const int b = batch_of(item), own = owned(item), count = list.count;
-      const float* grad = d.grad + static_cast<int64_t>(b) * p.S1 * d.width + key;
-      // this thread's gradients of a step: of its key, for the queries of its rows (0 behind the last query)
+      // kKeys: this thread's gradients of a step, of its key for the queries of its columns (0 behind the last query)
+      const float* grad = d.grad + static_cast<int64_t>(b) * p.S1 * d.width + own * kTile + row;
       auto gradients = [&](int i, float (&to)[kMine]) {
-        const int step = list.step[i], tile = kOwner == kQueries ? step : own, query0 = (kOwner == kQueries ? own : step) * d.queries + group * kCols / N1;
+        const int query0 = list.step[i] * kMine;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) to[k] = query0 + k < p.S1 ? __ldg(grad + static_cast<int64_t>(query0 + k) * d.width + tile * kTile) : 0.f;
+        for (int k = 0; k < kMine; ++k) to[k] = query0 + k < p.S1 ? __ldg(grad + static_cast<int64_t>(query0 + k) * d.width) : 0.f;
       };
-      float dw[kOwner == kQueries ? kCols : 1];
-#pragma unroll
-      for (int k = 0; k < (kOwner == kQueries ? kCols : 1); ++k) dw[k] = 0.f;
+      const int first = (group + kSlots - g % kSlots) % kSlots;   // this group's first step of the item
       float next[kMine];
-      gradients(0, next);
-      for (int i = 0; i < count; ++i, ++g) {
-        float gr[kMine], above[kMine];   // dz where z is above: nowhere without a gradient, whatever the weight is
+      if constexpr (kOwner == kKeys) {
+        if (first < count) gradients(first, next);
+      }
+      // kQueries: the weight of this thread's row
+      const int own_rows = min(kTile, (p.S1 - own * kMine) * N1);   // (kQueries)
+      const float weight = kOwner == kQueries && row < own_rows ? __ldg(p.w + (static_cast<int64_t>(b) * p.S1 + own * kMine) * N1 + row) : 0.f;
+      float2 dw = make_float2(0.f, 0.f), dw2 = make_float2(0.f, 0.f);
+      for (int i = first; i < count; i += kSlots) {
+        const int s = stage_of(g + i);
+        float gr[kMine];
+        if constexpr (kOwner == kKeys) {
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-          gr[k] = next[k];
-          above[k] = gr[k] != 0.f ? 0.f : INFINITY;
+          for (int k = 0; k < kMine; ++k) gr[k] = next[k];
+          if (i + kSlots < count) gradients(i + kSlots, next);
         }
-        if (i + 1 < count) gradients(i + 1, next);
-        ok = ok && wait_both(&z_full[g & 1], use(g), &dz_free[g & 1], before(g), g >= 2);
-        if (!ok) continue;
+        if (!wait(&z_full[group], turn(g + i))) { ok = false; break; }
         tc_fence_after();
-        const uint32_t dz = sDz + (g & 1) * kTileBytes + (group >> 1) * kChunk;
-        const float4* w4 = reinterpret_cast<const float4*>(s_w + (kOwner == kQueries ? kStages : g % kStages) * kTile + group * kCols);
+        const uint32_t z_at = tmem_base + kColZ + group * kTile + lane_base;
+        uint32_t v[2][32];
+        tmem_ld32(z_at, v[0]);
+        // what came beside the tile (only now: before Z of this step, the stage may be a lap behind)
+        ok = wait(&full[s], lap(g + i));   // (if not, this step still ends: a load is under way)
+        // kQueries: the gradients of this row's query for its keys; kKeys: the weights of its columns
+        const float4* side = reinterpret_cast<const float4*>(smem + kOffSide + s * kSideBytes) + (kOwner == kQueries ? row / N1 * (kTile / 4) : 0);
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 16) {
-          const int k = c0 / N1;   // which of this thread's queries
-          uint32_t v[16], w[8];
-          tmem_ld16(tmem_base + kColZ + (g & 1) * kTile + group * kCols + c0 + lane_base, v);
+        for (int c = 0; c < 4; ++c) {   // dZ takes columns of Z that have been read
+          uint32_t w[16];
           tmem_wait_ld();
+          if (c < 3) tmem_ld32(z_at + (c + 1) * 32, v[(c + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 wt = w4[c0 / 4 + j];
-            const float2 gg = make_float2(gr[k], gr[k]), lo = fmul2(gg, make_float2(wt.x, wt.y)), hi = fmul2(gg, make_float2(wt.z, wt.w));
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = side[c * 8 + j];
             float z[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) z[m] = __uint_as_float(v[4 * j + m]);
+            for (int m = 0; m < 4; ++m) z[m] = __uint_as_float(v[c & 1][4 * j + m]);
+            float2 lo = make_float2(f.x, f.y), hi = make_float2(f.z, f.w), scale;
             if constexpr (kOwner == kQueries) {
-              float* e = dw + c0 + 4 * j;
-              const float2 lo_w = ffma2(gg, make_float2(fmaxf(z[0], 0.f), fmaxf(z[1], 0.f)), make_float2(e[0], e[1]));
-              const float2 hi_w = ffma2(gg, make_float2(fmaxf(z[2], 0.f), fmaxf(z[3], 0.f)), make_float2(e[2], e[3]));
-              e[0] = lo_w.x; e[1] = lo_w.y; e[2] = hi_w.x; e[3] = hi_w.y;
+              dw = ffma2(lo, make_float2(fmaxf(z[0], 0.f), fmaxf(z[1], 0.f)), dw);
+              dw2 = ffma2(hi, make_float2(fmaxf(z[2], 0.f), fmaxf(z[3], 0.f)), dw2);
+              scale = make_float2(weight, weight);
+            } else {
+              scale = make_float2(gr[(32 * c + 4 * j) / N1], gr[(32 * c + 4 * j) / N1]);
             }
-            w[2 * j] = pack2<true>(z[0] > above[k] ? lo.x : 0.f, z[1] > above[k] ? lo.y : 0.f);
-            w[2 * j + 1] = pack2<true>(z[2] > above[k] ? hi.x : 0.f, z[3] > above[k] ? hi.y : 0.f);
+            lo = fmul2(lo, scale);
+            hi = fmul2(hi, scale);
+            w[2 * j] = pack2<true>(z[0] > 0.f ? lo.x : 0.f, z[1] > 0.f ? lo.y : 0.f);
+            w[2 * j + 1] = pack2<true>(z[2] > 0.f ? hi.x : 0.f, z[3] > 0.f ? hi.y : 0.f);
           }
-          const int unit = (group & 1) * 4 + c0 / 8;
-          st_shared_v4(dz + sw128_offset(key, unit), w[0], w[1], w[2], w[3]);
-          st_shared_v4(dz + sw128_offset(key, unit + 1), w[4], w[5], w[6], w[7]);
+          tmem_st16(z_at + c * 16, w);
         }
+        tmem_wait_st();
         tc_fence_before();
-        fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&z_free[g & 1]);
-          mbar_arrive(&dz_full[g & 1]);
-        }
+        if (lane == 0) mbar_arrive(&dz_full[group]);
+        if (!ok) break;
       }
-      if constexpr (kOwner == kQueries) {
-        // dw over the lanes (lane l ends with row l of the group), then over the four quarters
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const bool upper = lane & o;
-#pragma unroll
-          for (int k = 0; k < o; ++k) {
-            const float give = upper ? dw[k] : dw[k + o], mine = upper ? dw[k + o] : dw[k];
-            dw[k] = mine + __shfl_xor_sync(0xffffffffu, give, o);
-          }
-        }
-        s_dw[quarter * kTile + group * kCols + lane] = dw[0];
-        named_bar_sync(1, kWorkers * 32);
-        const int rows = min(kTile, (p.S1 - own * d.queries) * N1);
-        if (ok && tid < rows)
-          p.d_w[(static_cast<int64_t>(b) * p.S1 + own * d.queries) * N1 + tid] =
-              (s_dw[tid] + s_dw[kTile + tid]) + (s_dw[2 * kTile + tid] + s_dw[3 * kTile + tid]);
-      }
-      ok = ok && wait(own_done, n & 1);
-      if (ok) {
-        tc_fence_after();
-#pragma unroll 1
-        for (int c0 = 0; c0 < kCols; c0 += 16) {
-          uint32_t v[16];
-          tmem_ld16(tmem_base + kColAcc + (n & 1) * kTile + group * kCols + c0 + lane_base, v);
-          tmem_wait_ld();
-          const int first = own * kTile + group * kCols + c0, dim = quarter * 32 + lane;   // the sum's first column among the batch entry's rows or keys
-          const int limit = kOwner == kQueries ? p.S1 * N1 : p.S2;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            if (first + k >= limit) continue;
-            const int64_t at = (static_cast<int64_t>(b) * limit + first + k) * kD + dim;
-            if (kOwner == kQueries) reinterpret_cast<__nv_bfloat16*>(p.d_q)[at] = __float2bfloat16(__uint_as_float(v[k]));
-            else atomicAdd(p.d_k + at, __uint_as_float(v[k]));
-          }
-        }
-        tc_fence_before();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_free[n & 1]);
+      if (!ok) break;
+      g += count;
       done_with(n);
+      // dw by group, in the order of their first steps (which group has which varies).  Three items' worth: the list
+      // of n + 3 comes when every warp is done with that of n + 1, so behind its reading of n.
+      float* dw_at = s_dw + (n % kDwItems) * kSlots * kTile + row;
+      if constexpr (kOwner == kQueries) {
+        dw_at[first * kTile] = (dw.x + dw.y) + (dw2.x + dw2.y);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dw_full);
+      }
+      if ((g - 1) % kSlots != group) continue;
+      if (!wait(&dz_free[group], turn(g - 1))) { ok = false; break; }   // all MMAs up to the last step's are done
+      tc_fence_after();
+      auto read = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_free);
+      };
+      const uint32_t acc = tmem_base + kColAcc + lane_base;
+      if constexpr (kOwner == kQueries) {
+        uint32_t o[kD / 2];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(acc + c * 32, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[16 * c + k] = pack2<true>(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+        }
+        if (!wait(dw_full, n & 1)) { ok = false; break; }
+        float sum = dw_at[0];
+        for (int k = 1; k < kSlots; ++k) sum += dw_at[k * kTile];
+        read();
+        if (row < own_rows) {
+          const int64_t at = (static_cast<int64_t>(b) * p.S1 + own * kMine) * N1 + row;
+          p.d_w[at] = sum;
+          uint4* dq = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.d_q) + at * kD);
+#pragma unroll
+          for (int j = 0; j < kD / 8; ++j) dq[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+      } else {
+        float* dk = p.d_k + (static_cast<int64_t>(b) * p.S2 + own * kTile + row) * kD;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(acc + c * 32, v);
+          tmem_wait_ld();
+          if (c == 3) read();
+          if (own * kTile + row < p.S2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) red_add_v4(dk + c * 32 + 4 * j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+          __syncwarp();
+        }
+      }
     }
   }
   tc_fence_before();
@@ -489,11 +521,12 @@ int launch_both(const IndexerBwdParams& p, const ibd::Dense& d, const CUtensorMa
 }
 }  // namespace
 
-// Which kernel: the other one takes about 105 ps per (query, listed key), whatever the heads; these take 60 ps per (query, key that it may
-// see) with 64 heads, half and a quarter of that with 32 and 16, and 20 us more for G and three more launches.  Both counts as they are
-// in a causal step (keys up to S2 - S1 + t) with full lists.  Measured, other / these, us: 4096 queries x 4096 keys, lists of 2048:
-// 671 / 540, of 1024: 410 / 530; 4096 x 8192, 2048: 855 / 1416; 1024 x 4096, 2048: 223 / 278; 4096 x 1024, 512, 16 heads: 258 / 118; 2048 x 2048,
-// 2048, 32 heads: 251 / 121.  fp16 stays with the other kernel: its range needs a scale per query.
+// Which kernel: the other one takes about 100 ps per (query, listed key), whatever the heads; these take 8 ps per (query, key that it may see) for
+// G, 42 more with 64 heads, half and a quarter of that with 32 and 16, and 30 us for three more launches.  Both counts as they are
+// in a causal step (keys up to S2 - S1 + t) with full lists.  Measured, other / these, us (queries x keys, list): 64 heads: 4096 x 4096, 2048:
+// 670 / 480, 1024: 412 / 473; 4096 x 8192, 2048: 855 / 1220; 1024 x 4096, 2048: 224 / 232; 32 heads: 2048 x 2048, 2048: 251 / 129; 4096 x 8192,
+// 2048: 850 / 661; 16 heads: 4096 x 4096, 512: 254 / 205; 4096 x 1024, 512: 262 / 132.  fp16 stays with the other kernel: its range needs a
+// scale per query.
 static bool dense_preferred(const IndexerBwdParams& p, bool bf16) {
   if (!bf16 || p.D != ibd::kD || (p.N1 != 16 && p.N1 != 32 && p.N1 != 64)) return false;
   const long long B = p.B, S1 = p.S1, S2 = p.S2, K = p.K < p.S2 ? p.K : p.S2;
@@ -502,7 +535,7 @@ static bool dense_preferred(const IndexerBwdParams& p, bool bf16) {
   const long long first = S2 - S1 + 1;   // keys that query 0 may see
   const long long shorter = S1 > S2 || first >= K ? 0 : (K - first < S1 ? K - first : S1);   // queries that see fewer than K
   const long long listed = S1 * K - (shorter ? shorter * (2 * K - 2 * first - shorter + 1) / 2 : 0);
-  return B * listed * 105 > B * seen * 60 * p.N1 / 64 + 20 * 1000 * 1000;
+  return B * listed * 100 > B * seen * (8 + 42 * p.N1 / 64) + 30 * 1000 * 1000;
 }
 
 namespace {
@@ -524,7 +557,8 @@ size_t indexer_bwd_workspace_bytes(const IndexerBwdParams& p, bool bf16) { retur
 
 // Is a call that brought this workspace, 16-byte aligned, taken here?
 bool indexer_bwd_dense_fits(const IndexerBwdParams& p, bool bf16) {
-  return dense_preferred(p, bf16) && (reinterpret_cast<uintptr_t>(p.w) & 15u) == 0 && encode_tiled_fn() != nullptr;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.d_q) | reinterpret_cast<uintptr_t>(p.d_k);
+  return dense_preferred(p, bf16) && (bases & 15u) == 0 && encode_tiled_fn() != nullptr;
 }
 
 // *dirty_out: where the device says whether the call is left to launch_indexer_bwd.
@@ -536,8 +570,8 @@ int launch_indexer_bwd_dense(const IndexerBwdParams& p, void* workspace, const i
   Dense d;
   d.width = padded_width(p);
   d.tiles = d.width / kTile;
-  d.queries = kTile / p.N1;
-  d.blocks = (p.S1 + d.queries - 1) / d.queries;
+  const int queries = kTile / p.N1;   // per block of 128 rows
+  d.blocks = (p.S1 + queries - 1) / queries;
   // a key tile's blocks in parts: about eight items per SM, so that their unequal lengths even out
   int splits = (8 * sms + p.B * d.tiles - 1) / (p.B * d.tiles);
   if (splits > d.blocks) splits = d.blocks;
