@@ -1,6 +1,7 @@
 """B200 (sm_100a) kernels for the DeepSeek-sparse-attention hot path, behind the entry signatures of
 the TileLang-Ascend examples: lightning indexer -> top-k selector -> sparse MLA forward (+ decode,
-backward).  Python / PyTorch host code over a C-ABI CUDA library; there is no CPU fallback."""
+backward); what feeds the indexer and its caches (norm + rotation) and what trains it (distillation).
+Python / PyTorch host code over a C-ABI CUDA library; there is no CPU fallback."""
 from . import _lib
 from .deepseek_mla import flashattn_mla_decode, mla_decode, mla_decode_tilelang, run_mla_decode
 from .distillation import (lightning_indexer_bwd_raw, lightning_indexer_distillation, topk_distillation, topk_distillation_bwd_raw,
