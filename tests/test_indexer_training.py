@@ -246,6 +246,32 @@ def test_gradient_of_lists_that_hold_most_keys(B, S1, S2, N1, K):
 
 
 @pytest.mark.gpu
+def test_gradient_of_very_many_queries():
+    """More than 2^16 blocks of 128 (query, head) rows, whose places no 16-bit number holds."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    S1, S2, N1 = 135001, 96, 64
+    query = torch.randn((1, S1, N1, 128), generator=g, device="cuda", dtype=torch.bfloat16)
+    key = torch.randn((1, S2, 1, 128), generator=g, device="cuda", dtype=torch.bfloat16)
+    weights = torch.randn((1, S1, N1), generator=g, device="cuda")
+    indices = torch.arange(S2, dtype=torch.int32, device="cuda").expand(1, S1, 1, S2).contiguous()
+    d_values = torch.randn((1, S1, 1, S2), generator=g, device="cuda")
+    dq, dk, dw = dsa.lightning_indexer_bwd_raw(query, key, weights, indices, d_values)
+    keys, want_k = key[0, :, 0].double(), torch.zeros((S2, 128), dtype=torch.float64, device="cuda")
+    for s in range(0, S1, 5000):
+        q, gr, w = query[0, s:s + 5000].double(), d_values[0, s:s + 5000, 0].double(), weights[0, s:s + 5000].double()
+        z = q @ keys.T
+        want_w = (z.clamp(min=0) * gr[:, None]).sum(2)
+        dz = (z > 0) * gr[:, None] * w[:, :, None]
+        want_q = dz @ keys
+        want_k += torch.einsum("shk,shd->kd", dz, q)
+        assert float((dq[0, s:s + 5000].double() - want_q).norm() / want_q.norm()) <= 2 * 2.0 ** -8
+        assert float((dw[0, s:s + 5000].double() - want_w).norm() / want_w.norm()) <= 2.0 ** -18
+    # dz rounded once, of every term
+    assert float((dk[0, :, 0].double() - want_k).norm() / want_k.norm()) <= 2.0 ** -8
+    check_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("where", ["query", "key", "weights"])
 def test_unlisted_values_whose_products_overflow(where):
     """Finite, but with infinite products: rows that take part in no listed pair leave the gradients as they are."""

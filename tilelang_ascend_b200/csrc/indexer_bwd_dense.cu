@@ -39,7 +39,7 @@ constexpr int kWorkers = 4 * kSlots, kLoadWarp = kWorkers, kZWarp = kWorkers + 1
 constexpr int kUsers = kWorkers + 3;
 struct Steps {
   int item, count;               // item -1: no more
-  int pad[2];
+  int first, pad;                // tile `first` + step
   uint16_t step[kMaxSteps];
 };
 constexpr int kDwItems = 3;
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
           for (int k = 0; k < kMine; ++k) any |= __ldg(flags + static_cast<int64_t>(min(block * kMine + k, p.S1 - 1)) * d.tiles + tile);
         }
         const uint32_t bits = __ballot_sync(0xffffffffu, any != 0);
-        if (any) list.step[count + __popc(bits & ((1u << lane) - 1))] = static_cast<uint16_t>(s);
+        if (any) list.step[count + __popc(bits & ((1u << lane) - 1))] = static_cast<uint16_t>(s - first);
         count += __popc(bits);
       }
       if (!count) {
@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
       if (lane == 0) {
         list.item = item;
         list.count = count;
+        list.first = first;
         mbar_arrive(&list_full[n & 1]);
       }
       __syncwarp();
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
         const int s = stage_of(g);
         if (g >= kStages && !wait(&empty[s], lap(g) ^ 1u)) { ok = false; break; }
         if (lane == 0) {
-          const int tile = list.step[i];
+          const int tile = list.first + list.step[i];
           const uint32_t bar = smem_u32(&full[s]), side = sSide + s * kSideBytes;
           // beside a key tile the gradients of the own block's queries, beside a block of rows their head weights
           const uint32_t side_bytes = kOwner == kQueries ? static_cast<uint32_t>(own_queries) * kTile * 4u : static_cast<uint32_t>(min(kTile, p.S1 * N1 - tile * kTile)) * 4u;
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
       // kKeys: this thread's gradients of a step, of its key for the queries of its columns (0 behind the last query)
       const float* grad = d.grad + static_cast<int64_t>(b) * p.S1 * d.width + own * kTile + row;
       auto gradients = [&](int i, float (&to)[kMine]) {
-        const int query0 = list.step[i] * kMine;
+        const int query0 = (list.first + list.step[i]) * kMine;
 #pragma unroll
         for (int k = 0; k < kMine; ++k) to[k] = query0 + k < p.S1 ? __ldg(grad + static_cast<int64_t>(query0 + k) * d.width) : 0.f;
       };
