@@ -294,7 +294,30 @@ def test_repeatable_captured_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(captured, step()))
 
 
+@pytest.mark.gpu
+def test_gradient_of_one_side_alone():
+    """A side without a gradient is left out, whatever else is given for it."""
+    g = torch.Generator().manual_seed(5)
+    q, k, d_q, d_k = (torch.randn((2, 9, h, 64), generator=g).to(torch.bfloat16).cuda() for h in (4, 1, 4, 1))
+    pos, f = torch.arange(18, dtype=torch.int32).view(2, 9).cuda(), torch.rand(16, generator=g).cuda()
+    w = torch.rand(64, generator=g).cuda()
+    how = dict(q_norm="rms", k_norm="layer", q_weight=w, k_weight=w, k_bias=w)
+    both = dsa.qk_norm_rope_bwd_raw(d_q, d_k, q, k, pos, f, **how)
+    keys, queries = dsa.qk_norm_rope_bwd_raw(None, d_k, q, k, pos, f, **how), dsa.qk_norm_rope_bwd_raw(d_q, None, q, k, pos, f, **how)
+    assert all(keys[i] is None for i in (0, 2, 3)) and all(torch.equal(keys[i], both[i]) for i in (1, 4, 5))
+    assert all(queries[i] is None for i in (1, 3, 4, 5)) and all(torch.equal(queries[i], both[i]) for i in (0, 2))
+
+
 # --------------------------------------------------------------------------------------------------------- refusals
+def test_refusals_of_slots_and_of_a_side_alone():
+    q, k = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)
+    pos, f, w = torch.zeros(2, 3, dtype=torch.int32), torch.ones(16), torch.ones(64)
+    with pytest.raises(ValueError, match="slots"):
+        dsa.qk_norm_rope_cached(q, k, pos, f, torch.zeros(2, 8, 1, 64, dtype=torch.bfloat16), [[0, 1, 2], [3, 4, 5]])
+    with pytest.raises(ValueError, match="no CPU path"):   # (everything else is in order)
+        dsa.qk_norm_rope_bwd_raw(None, k, q, k, pos, f, q_norm="rms", q_weight=w, k_norm="rms", k_weight=w)
+
+
 def test_refusals():
     q, k = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)
     pos, f = torch.zeros(2, 3, dtype=torch.int32), torch.ones(16)

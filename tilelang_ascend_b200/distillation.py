@@ -226,6 +226,6 @@ def lightning_indexer_distillation(query, key, weights, indices, values, teacher
     query [B,S1,N1,128], key [B,S2,1,128] bf16 / fp16, weights [B,S1,N1] fp32 (at most 64 heads); ``indices`` and ``values``
     [B,S1,1,K] are what :func:`lightning_indexer_raw` returned for them (int32, -1 pads; fp32 scores, -inf there); ``teacher``
     [B,S1,1,K] fp32 its entries, e.g. from :func:`sparse_mla_key_weights`.  ``values`` are taken as the scores of these inputs: no
-    gradient flows through them or through the teacher.  An entry takes part when its value is not -inf and its index lies in
-    [0, S2)."""
+    gradient flows through them or through the teacher.  An entry takes part when its value is not -inf; one whose index lies
+    outside [0, S2) must have the value -inf, as it has there."""
     return LightningIndexerDistillationFunction.apply(query, key, weights, indices, values, teacher, teacher_kind, float(temperature))

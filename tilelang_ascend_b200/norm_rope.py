@@ -190,7 +190,7 @@ def qk_norm_rope_bwd_raw(d_q, d_k, q, k, positions, inv_freq, *, rope_start: int
             if norm is not None and (x is None or d_y.shape != x.shape or d_y.dtype != x.dtype):
                 raise ValueError(f"{name} {tuple(d_y.shape)} {d_y.dtype} does not fit the forward's input")
     rows = tuple(None if d_y is None else (d_y if norm is None else x) for d_y, x, norm in ((d_q, q, q_norm), (d_k, k, k_norm)))
-    params = ((q_weight, q_bias), (k_weight, k_bias))
+    params = tuple((None, None) if d_y is None else pair for d_y, pair in ((d_q, (q_weight, q_bias)), (d_k, (k_weight, k_bias))))
     call = _Call(rows, positions, inv_freq, rope_start, interleaved, rope_scale, (q_norm, k_norm), params, norm_dim, eps, others=((d_q, "d_q"), (d_k, "d_k")))
     call.require_cuda()
     (dq, dk), (dqp, dkp) = _backward(call, (d_q, d_k), rows, params, positions, inv_freq, (True, True), ((True, True), (True, True)))
@@ -225,6 +225,8 @@ def qk_norm_rope_cached(q, k, positions, inv_freq, key_cache, slots, *, key_cach
         raise ValueError("k must be given")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, q_bias, k_weight, k_bias)):
         raise ValueError("qk_norm_rope_cached has no gradient; use qk_norm_rope, or call it under torch.no_grad()")
+    if not isinstance(slots, torch.Tensor):
+        raise ValueError("slots must be an int32 or int64 tensor")
     caches = ((key_cache, "key_cache"),) if key_cache_rope is None else ((key_cache, "key_cache"), (key_cache_rope, "key_cache_rope"))
     for t, name in caches:
         if not isinstance(t, torch.Tensor) or t.dim() != 4 or not t.is_contiguous():
