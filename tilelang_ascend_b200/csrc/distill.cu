@@ -12,7 +12,7 @@
 // their digits; all sums in fp32.  (Entries kept in registers and three passes over them: 4096 lists of 2048 forward 87 us; exact
 // logarithms and divisions per entry were half of that.)  Backward with indices: a block owns 8192 columns of a row, asks for them,
 // adds the listed entries of its columns up in shared memory meanwhile (a column may be listed more than once) and writes the columns.
-// Measured, fp32: 1024 rows of 131072 with 2048 entries: forward 111 us (4.8 TB/s), backward 198 (5.4 TB/s); 4096 lists of 2048: 20 and 13 us
+// Measured, fp32: 1024 rows of 131072 with 2048 entries: forward 107 us (5.0 TB/s), backward 194 (5.5 TB/s); 4096 lists of 2048: 20 and 13 us
 // (out of L2 in part).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -483,14 +483,16 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const __grid_constant_
 
 // -------------------------------------------------------------------------------------------------
 // backward with indices: block = (row, kChunk of its columns).  kWide: rows in aligned 16-byte units, else element by element.
+// Last rows first: those are still in L2 when the forward has just read them (1024 rows of 131072 fp32: 198 -> 194 us, and the next
+// forward finds the first rows: 111 -> 107).
 // -------------------------------------------------------------------------------------------------
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(dt::kListedThreads) distill_bwd_listed_kernel(const __grid_constant__ DistillParams p, const int parts) {
   using namespace dt;
   __shared__ __align__(16) float acc[kChunk];
   constexpr int kN = kWide ? Vec<T>::kN : 1, kUnits = kPerThread / kN;
-  const int64_t r = blockIdx.x / parts;
-  const int c0 = static_cast<int>(blockIdx.x - r * parts) * kChunk, n = min(p.V - c0, kChunk);
+  const int64_t block = gridDim.x - 1 - blockIdx.x, r = block / parts;
+  const int c0 = static_cast<int>(block - r * parts) * kChunk, n = min(p.V - c0, kChunk);
   const int tid = threadIdx.x;
   const T* src = static_cast<const T*>(p.student) + r * p.row_stride + c0;
   T* out = static_cast<T*>(p.d_student) + r * p.V + c0;
