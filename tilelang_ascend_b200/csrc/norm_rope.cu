@@ -11,7 +11,9 @@
 // usual sizes (a warp per row left a quarter of its lanes idle at 576 dims and had one row on its way: 4096 tokens x 129 rows
 // of 576 dims 264 us).  A block owns a tile of tokens x heads; the cosines and sines of its tokens are made once per block, the
 // angle as an exact product reduced in 64 bits (a far position times a frequency has no fraction left in 32).
-// That call takes 195 us now, 6.2 TB/s.  Forward and backward of 4096 tokens x 65 rows of 128 dims, layer norm on one of them: 96 us.
+// That call takes 188 us now, 6.5 TB/s.  Short rows are bound by their instructions (390 per warp and four rows of 128 dims with a division
+// per row and the lanes' angles in the same banks): forward and backward of 4096 tokens x 65 rows of 128 dims, layer norm on one of
+// them, 96 us then, 74 now.
 // Everything is computed in fp32 and rounded once, on the store.  The gradient of rows without a norm is the forward with the angles
 // turned round.
 //
@@ -93,24 +95,47 @@ __device__ __forceinline__ long long out_row(const RopeSide& sd, int token, int 
   return slot >= 0 && slot < sd.y_slots ? slot * sd.H + head : -1;
 }
 
+// Where angle i of a token's `half` sits in shared memory: the 16-byte pieces (two angles) that make up a unit's angles -- four, or with
+// interleaved pairs two -- lie apart, so that lanes with neighbouring units read neighbouring pieces.  (All of a unit's angles side
+// by side: the lanes' reads met in a quarter of the banks.)
+__device__ __forceinline__ int turn_slot(int i, int half, int interleaved) {
+  const int log_pieces = interleaved ? 1 : 2, piece = (i >> 1) & ((1 << log_pieces) - 1), unit = (i >> 1) >> log_pieces;
+  return 2 * (piece * (half >> (log_pieces + 1)) + unit) + (i & 1);
+}
+// The angles of a block's tokens.
+__device__ __forceinline__ void make_turns(const NormRopeParams& p, float2* turns, int token0, int tokens) {
+  const int half = p.R >> 1;
+  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+    const int tk = i / half, pair = i - tk * half;
+    turns[tk * half + turn_slot(pair, half, p.interleaved)] = turn_of(p, position_of(p, token0 + tk), p.inv_freq[pair]);
+  }
+}
+
 // The rotation of unit e0 .. e0 + 7 (dims relative to rope_start) of a row: v = this unit, o = its partner unit (halves only).
 __device__ __forceinline__ void rotate8(float (&v)[8], const float (&o)[8], const float2* turns, int e0, int half, bool interleaved) {
+  const float4* t4 = reinterpret_cast<const float4*>(turns);
   if (interleaved) {
+    t4 += e0 >> 3;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 t = turns[(e0 >> 1) + j];
-      const float a = v[2 * j], b = v[2 * j + 1];
-      v[2 * j] = a * t.x - b * t.y;
-      v[2 * j + 1] = b * t.x + a * t.y;
+    for (int j = 0; j < 2; ++j) {
+      const float4 t = t4[j * (half >> 2)];
+      const float c[2] = {t.x, t.z}, s[2] = {t.y, t.w};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float a = v[4 * j + 2 * k], b = v[4 * j + 2 * k + 1];
+        v[4 * j + 2 * k] = a * c[k] - b * s[k];
+        v[4 * j + 2 * k + 1] = b * c[k] + a * s[k];
+      }
     }
   } else {
     const bool second = e0 >= half;
-    const int i0 = second ? e0 - half : e0;
+    t4 += (second ? e0 - half : e0) >> 3;
     const float sign = second ? 1.f : -1.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 t = turns[i0 + j];
-      v[j] = v[j] * t.x + o[j] * (sign * t.y);
+    for (int j = 0; j < 4; ++j) {
+      const float4 t = t4[j * (half >> 3)];
+      v[2 * j] = v[2 * j] * t.x + o[2 * j] * (sign * t.y);
+      v[2 * j + 1] = v[2 * j + 1] * t.z + o[2 * j + 1] * (sign * t.w);
     }
   }
 }
@@ -118,6 +143,35 @@ __device__ __forceinline__ void rotate8(float (&v)[8], const float (&o)[8], cons
 struct Tile {
   int side, token0, head0, tokens, heads;
 };
+// A group's rows of a tile, `step` rows apart: their tokens and heads without a division each.
+struct Walk {
+  int tk, head, step_tk, step_head;
+  __device__ __forceinline__ Walk(const Tile& t, int row, int step) {
+    tk = row / t.heads;
+    head = row - tk * t.heads;
+    step_tk = step_head = 0;
+    if (t.tokens * t.heads > step) {   // (there is a next one)
+      step_tk = step / t.heads;
+      step_head = step - step_tk * t.heads;
+    }
+  }
+  __device__ __forceinline__ void next(const Tile& t) {
+    tk += step_tk;
+    head += step_head;
+    if (head >= t.heads) { head -= t.heads; ++tk; }
+  }
+};
+// Element 0 of the row of a tile's token number tk and head: b0 and s0 are those of its first token.
+template <typename T>
+__device__ __forceinline__ const T* row_in(const RowView& v, const Tile& t, int S, int b0, int s0, int tk, int head) {
+  int b = b0, s = s0 + tk;
+  if (s >= S) {   // (few tiles reach into the next sequence)
+    const int more = s / S;
+    b += more;
+    s -= more * S;
+  }
+  return static_cast<const T*>(v.base) + b * v.stride_b + s * v.stride_s + (t.head0 + head) * v.stride_h;
+}
 __device__ __forceinline__ Tile tile_of(const NormRopeParams& p, int block) {
   Tile t;
   t.side = block >= p.side[0].blocks;
@@ -136,10 +190,12 @@ __device__ __forceinline__ Tile tile_of(const NormRopeParams& p, int block) {
 // -------------------------------------------------------------------------------------------------
 // forward, 16-byte units
 // -------------------------------------------------------------------------------------------------
+// (blocks per SM, in registers: short rows keep few bytes per thread on their way and need more threads: rows of 128 dims, the call above:
+// four blocks 80 us, five 76, six 80)
 template <typename T, int G, int NV>
-__global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(nr::kThreads, NV <= 2 ? 5 : 3) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   using namespace nr;
-  extern __shared__ float2 turns[];                       // [tile_tokens][R / 2]
+  extern __shared__ __align__(16) float2 turns[];         // [tile_tokens][R / 2]
   __shared__ __align__(16) float sw[kMaxNormDim], sb[kMaxNormDim];
   const Tile t = tile_of(p, blockIdx.x);
   const RopeSide& sd = p.side[t.side];
@@ -147,20 +203,20 @@ __global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid
   constexpr int kGroups = kThreads / G;
   const int units = p.D >> 3, half = p.R >> 1, rows = t.tokens * t.heads;
 
+  const int b0 = t.token0 / p.S, s0 = t.token0 - b0 * p.S;
+  Walk at(t, group, kGroups);
+  const T* x = nullptr;   // this group's row
   uint4 raw[NV];
-  auto fetch = [&](int row) {
-    const T* x = row_of<T>(sd.x, p.S, t.token0 + row / t.heads, t.head0 + row % t.heads);
+  auto fetch = [&]() {
+    x = row_in<T>(sd.x, t, p.S, b0, s0, at.tk, at.head);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (lane + G * i < units) raw[i] = ld_stream(x + (lane + G * i) * 8);
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) raw[i] = make_uint4(0, 0, 0, 0);   // (units beyond the row stay zero)
-  if (group < rows) fetch(group);   // the first row travels while the angles are made
-  for (int i = tid; i < t.tokens * half; i += kThreads) {
-    const int tk = i / half;
-    turns[i] = turn_of(p, position_of(p, t.token0 + tk), p.inv_freq[i - tk * half]);
-  }
+  if (group < rows) fetch();   // the first row travels while the angles are made
+  make_turns(p, turns, t.token0, t.tokens);
   if (sd.norm)
     for (int i = tid; i < p.norm_dim; i += kThreads) {
       sw[i] = sd.weight ? param_at<T>(sd.weight, sd.param_fp32, i) : 1.f;
@@ -169,11 +225,10 @@ __global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid
   __syncthreads();
 
   // (groups of one warp take the same number of turns through the loop, so that its shuffles see all lanes)
-  for (int row0 = 0; row0 < rows; row0 += kGroups) {
-    const int row = row0 + group;
-    const bool live = row < rows;
-    const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
-    if (row0 && live) fetch(row);
+  for (int row0 = 0; row0 < rows; row0 += kGroups, at.next(t)) {
+    const bool live = row0 + group < rows;
+    const int tk = live ? at.tk : 0;
+    if (row0 && live) fetch();
     float mean = 0.f, rstd = 1.f;
     if (sd.norm) {
       if (sd.norm == kNormLayer) {
@@ -205,7 +260,9 @@ __global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid
         for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd * sw[e + j] + sb[e + j];
       }
     };
-    const long long orow = live ? out_row(sd, token, head) : -1;
+    const long long orow = live ? out_row(sd, t.token0 + at.tk, t.head0 + at.head) : -1;
+    T* const y_lo = static_cast<T*>(sd.y) + orow * sd.split;
+    T* const y_hi = sd.split < p.D ? static_cast<T*>(sd.y_tail) + (orow * (p.D - sd.split) - sd.split) : y_lo;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = (lane + G * i) * 8, r = e - p.rope_start;
@@ -224,17 +281,14 @@ __global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid
             w.z = __shfl_xor_sync(0xffffffffu, raw[i].z, p.partner_xor);
             w.w = __shfl_xor_sync(0xffffffffu, raw[i].w, p.partner_xor);
           } else if (live && turned) {   // ... read once more, from L2
-            w = __ldg(reinterpret_cast<const uint4*>(row_of<T>(sd.x, p.S, token, head) + pe));
+            w = __ldg(reinterpret_cast<const uint4*>(x + pe));
           }
           unpack8<T>(w, o);
           if (turned) norm8(o, pe);
         }
         if (turned) rotate8(v, o, turns + tk * half, r, half, p.interleaved);
       }
-      if (orow >= 0 && e < p.D) {
-        T* y = e < sd.split ? static_cast<T*>(sd.y) + orow * sd.split + e : static_cast<T*>(sd.y_tail) + orow * (p.D - sd.split) + (e - sd.split);
-        *reinterpret_cast<uint4*>(y) = pack8<T>(v);
-      }
+      if (orow >= 0 && e < p.D) *reinterpret_cast<uint4*>((e < sd.split ? y_lo : y_hi) + e) = pack8<T>(v);
     }
   }
 }
@@ -246,7 +300,7 @@ __global__ void __launch_bounds__(nr::kThreads, 3) norm_rope_kernel(const __grid
 template <typename T, int G, int NV>
 __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
   using namespace nr;
-  extern __shared__ float2 turns[];
+  extern __shared__ __align__(16) float2 turns[];
   __shared__ __align__(16) float sw[kMaxNormDim], sdw[kMaxNormDim], sdb[kMaxNormDim];
   const RopeSide& sd = p.side[0];
   const int tid = threadIdx.x, lane = tid % G, group = tid / G;
@@ -266,23 +320,22 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
     const Tile t = tile_of(p, tile);
     const int rows = t.tokens * t.heads;
     __syncthreads();   // the last tile's angles have been used
-    for (int i = tid; i < t.tokens * half; i += kThreads) {
-      const int tk = i / half;
-      turns[i] = turn_of(p, position_of(p, t.token0 + tk), p.inv_freq[i - tk * half]);
-    }
+    make_turns(p, turns, t.token0, t.tokens);
     __syncthreads();
-    for (int row0 = 0; row0 < rows; row0 += kGroups) {
-      const int row = row0 + group;
-      const bool live = row < rows;
-      const int tk = live ? row / t.heads : 0, head = live ? t.head0 + row - tk * t.heads : 0, token = t.token0 + tk;
-      const T* dy = row_of<T>(sd.dy, p.S, token, head);
+    const int b0 = t.token0 / p.S, s0 = t.token0 - b0 * p.S;
+    Walk at(t, group, kGroups);
+    for (int row0 = 0; row0 < rows; row0 += kGroups, at.next(t)) {
+      const bool live = row0 + group < rows;
+      const int tk = live ? at.tk : 0, head = live ? at.head : 0;
+      const T* dy = row_in<T>(sd.dy, t, p.S, b0, s0, tk, head);
+      const T* x_row = row_in<T>(sd.x, t, p.S, b0, s0, tk, head);
       float v[NV][8], x[NV][8];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         uint4 w = make_uint4(0, 0, 0, 0), wx = w;
         if (live && lane + G * i < units) {
           w = ld_stream(dy + (lane + G * i) * 8);
-          if ((lane + G * i) * 8 < p.norm_dim) wx = ld_stream(row_of<T>(sd.x, p.S, token, head) + (lane + G * i) * 8);
+          if ((lane + G * i) * 8 < p.norm_dim) wx = ld_stream(x_row + (lane + G * i) * 8);
         }
         unpack8<T>(w, v[i]);
         unpack8<T>(wx, x[i]);
@@ -339,7 +392,7 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
           for (int j = 0; j < 8; ++j) v[i][j] = rstd * (v[i][j] - gn * x[i][j] - gs);
         }
       if (live) {
-        T* dx = static_cast<T*>(sd.y) + (static_cast<long long>(token) * sd.H + head) * p.D;
+        T* dx = static_cast<T*>(sd.y) + (static_cast<long long>(t.token0 + tk) * sd.H + t.head0 + head) * p.D;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (lane + G * i < units) *reinterpret_cast<uint4*>(dx + (lane + G * i) * 8) = pack8<T>(v[i]);
