@@ -12,7 +12,7 @@
 // first operand there.  What bounds a step is the way from Z to dZ to the sum's MMAs (about 3900 clocks, of which the two
 // products are 1024), so three steps are under way: three places for Z, each with four warps that turn Z into dZ all by themselves
 // (no barrier among them), and the group that has an item's last step reads the sum out while the others go on.  Measured for 4096 queries x 2048
-// of 4096 keys, 64 heads: kQueries 214 and kKeys 224 us (310 TFLOP/s of listed pairs each); with dZ in shared memory and all 16 warps at one
+// of 4096 keys, 64 heads: kQueries 206 and kKeys 207 us (1370 TFLOP/s of what they multiply); with dZ in shared memory and all 16 warps at one
 // step 257 and 244, of which the MMAs and the loads were not the bound (left out, the time stayed), the warps' 3200 clocks for two steps were.
 // Tiles are dense, so they come by TMA, without indices; (block, tile) pairs without a listed key are skipped by the flags (the upper
 // half of a causal step).
@@ -64,6 +64,26 @@ __device__ __forceinline__ void red_add_v4(float* dst, uint32_t a, uint32_t b, u
                : "memory");
 }
 
+// Four lanes' four 16-byte pieces transposed: piece j of lane l becomes piece l of lane j (within the lanes 4 i .. 4 i + 3).  Rows of which a
+// lane has one each then leave in 64-byte pieces, eight rows per request instead of thirty-two.
+__device__ __forceinline__ void quad_transpose(uint32_t* c, int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a & bit) continue;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t &lo = c[4 * a + w], &hi = c[4 * (a + bit) + w];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, bit);
+        lo = up ? got : lo;
+        hi = up ? hi : got;
+      }
+    }
+  }
+}
+
 struct Dense {
   const int* dirty;       // not 0: q, k or w hold what must not be multiplied by 0; nothing is done
   int* next;              // [2] items handed out so far
@@ -71,7 +91,7 @@ struct Dense {
   const uint8_t* flags;   // [B, S1, width / 128]
   int width, tiles;       // S2 rounded up to 128; width / 128
   int blocks;             // of a batch entry's queries
-  int splits, per_split;  // kKeys: parts a key tile's blocks are walked in
+  int big, per_big, small, per_small;   // kKeys: a key tile's blocks are walked in `big` parts of per_big, then `small` ones of per_small
 };
 }  // namespace ibd
 
@@ -203,10 +223,13 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(&list_free[n & 1]);
   };
-  const int per_batch = kOwner == kQueries ? d.blocks : d.tiles * d.splits, items = p.B * per_batch;
+  const int per_batch = kOwner == kQueries ? d.blocks : d.tiles * (d.big + d.small), items = p.B * per_batch;
   // an item's batch entry, and the block of rows or the key tile that it owns
   auto batch_of = [&](int item) { return item / per_batch; };
-  auto owned = [&](int item) { return kOwner == kQueries ? item % per_batch : item % per_batch / d.splits; };
+  auto owned = [&](int item) {
+    const int i = item % per_batch, most = d.tiles * d.big;
+    return kOwner == kQueries ? i : i < most ? i / d.big : (i - most) / d.small;
+  };
 
   if (warp == kListWarp) {
     // ================================ which tiles an item walks, one item ahead =====================
@@ -221,8 +244,17 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
       if (n >= 2 && !wait(&list_free[n & 1], before(n))) { ok = false; break; }
       Steps& list = lists[n & 1];
       const int b = batch_of(item), own = owned(item);
-      const int first = kOwner == kQueries ? 0 : (item % d.splits) * d.per_split;
-      const int last = kOwner == kQueries ? d.tiles : min(d.blocks, first + d.per_split);
+      int first = 0, last = d.tiles;
+      if constexpr (kOwner == kKeys) {
+        const int i = item % per_batch, most = d.tiles * d.big;
+        if (i < most) {
+          first = i % d.big * d.per_big;
+          last = first + d.per_big;
+        } else {
+          first = d.big * d.per_big + (i - most) % d.small * d.per_small;
+          last = min(d.blocks, first + d.per_small);
+        }
+      }
       const uint8_t* flags = d.flags + static_cast<int64_t>(b) * p.S1 * d.tiles;
       int count = 0;
       for (int s0 = first; s0 < last; s0 += 32) {
@@ -471,24 +503,32 @@ __global__ void __launch_bounds__(ibd::kThreads, 1)
         float sum = dw_at[0];
         for (int k = 1; k < kSlots; ++k) sum += dw_at[k * kTile];
         read();
-        if (row < own_rows) {
-          const int64_t at = (static_cast<int64_t>(b) * p.S1 + own * kMine) * N1 + row;
-          p.d_w[at] = sum;
-          uint4* dq = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.d_q) + at * kD);
+        const int64_t row0 = (static_cast<int64_t>(b) * p.S1 + own * kMine) * N1;
+        if (row < own_rows) p.d_w[row0 + row] = sum;
+        uint4* dq = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.d_q) + (row0 + (row & ~3)) * kD) + (lane & 3);
 #pragma unroll
-          for (int j = 0; j < kD / 8; ++j) dq[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        for (int h = 0; h < 4; ++h) {   // 32 dims
+          quad_transpose(o + 16 * h, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((row & ~3) + j < own_rows) dq[j * (kD / 8) + 4 * h] = make_uint4(o[16 * h + 4 * j], o[16 * h + 4 * j + 1], o[16 * h + 4 * j + 2], o[16 * h + 4 * j + 3]);
         }
       } else {
-        float* dk = p.d_k + (static_cast<int64_t>(b) * p.S2 + own * kTile + row) * kD;
+        const int row4 = own * kTile + (row & ~3);
+        float* dk = p.d_k + (static_cast<int64_t>(b) * p.S2 + row4) * kD + 4 * (lane & 3);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t v[32];
           tmem_ld32(acc + c * 32, v);
           tmem_wait_ld();
           if (c == 3) read();
-          if (own * kTile + row < p.S2) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) red_add_v4(dk + c * 32 + 4 * j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int h = 0; h < 2; ++h) {   // 16 dims
+            uint32_t* u = v + 16 * h;
+            quad_transpose(u, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (row4 + j < p.S2) red_add_v4(dk + j * kD + c * 32 + 16 * h, u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
           }
           __syncwarp();
         }
@@ -511,7 +551,7 @@ int launch_owner(const IndexerBwdParams& p, const ibd::Dense& d, const CUtensorM
   auto kern = indexer_bwd_dense_kernel<kOwner, N1>;
   const cudaError_t e = ensure_dynamic_smem(kern, dev, static_cast<int>(ibd::kSmemBytes));
   if (e != cudaSuccess) return static_cast<int>(e);
-  const long long items = static_cast<long long>(p.B) * (kOwner == kQueries ? d.blocks : d.tiles * d.splits);
+  const long long items = static_cast<long long>(p.B) * (kOwner == kQueries ? d.blocks : d.tiles * (d.big + d.small));
   kern<<<static_cast<unsigned>(items < sms ? items : sms), ibd::kThreads, ibd::kSmemBytes, stream>>>(p, d, q_map, k_map);
   return static_cast<int>(cudaGetLastError());
 }
@@ -573,12 +613,15 @@ int launch_indexer_bwd_dense(const IndexerBwdParams& p, void* workspace, const i
   d.tiles = d.width / kTile;
   const int queries = kTile / p.N1;   // per block of 128 rows
   d.blocks = (p.S1 + queries - 1) / queries;
-  // a key tile's blocks in parts: about eight items per SM, so that their unequal lengths even out
-  int splits = (8 * sms + p.B * d.tiles - 1) / (p.B * d.tiles);
-  if (splits > d.blocks) splits = d.blocks;
-  d.per_split = (d.blocks + splits - 1) / splits;
-  if (d.per_split > kMaxSteps) d.per_split = kMaxSteps;
-  d.splits = (d.blocks + d.per_split - 1) / d.per_split;
+  // A key tile's blocks in parts, as many as make about six items per SM; the last quarter of them in smaller ones, handed out last, so
+  // that the SMs end together (all of one size, eight per SM: 224 us; so 212, with four per SM 240, with half of them small 232).
+  int parts_of_tile = (6 * sms + p.B * d.tiles - 1) / (p.B * d.tiles);
+  if (parts_of_tile > d.blocks) parts_of_tile = d.blocks;
+  d.per_big = (d.blocks + parts_of_tile - 1) / parts_of_tile;
+  if (d.per_big > kMaxSteps) d.per_big = kMaxSteps;
+  d.big = 3 * (d.blocks / 4) / d.per_big;
+  d.per_small = (d.per_big + 3) / 4;
+  d.small = (d.blocks - d.big * d.per_big + d.per_small - 1) / d.per_small;
   const Layout l = layout(p);
   float* G = static_cast<float*>(workspace);
   uint8_t* flags = static_cast<uint8_t*>(workspace) + l.flags;
