@@ -12,7 +12,7 @@
 // their digits; all sums in fp32.  (Entries kept in registers and three passes over them: 4096 lists of 2048 forward 87 us; exact
 // logarithms and divisions per entry were half of that.)  Backward with indices: a block owns 8192 columns of a row, asks for them,
 // adds the listed entries of its columns up in shared memory meanwhile (a column may be listed more than once) and writes the columns.
-// Measured, fp32: 1024 rows of 131072 with 2048 entries: forward 107 us (5.0 TB/s), backward 194 (5.5 TB/s); 4096 lists of 2048: 20 and 13 us
+// Measured, fp32: 1024 rows of 131072 with 2048 entries: forward 107 to 111 us (4.9 TB/s), backward 194 (5.5 TB/s); 4096 lists of 2048: 20 and 13 us
 // (out of L2 in part).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
