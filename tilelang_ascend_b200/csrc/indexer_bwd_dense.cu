@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256)
   auto put = [&](int key, float g) {
     const int c = key - c0;
     if (key >= 0 && key < p.S2 && c >= 0 && c < n) {
-      atomicAdd(&acc[c], g);   // (a key listed twice counts twice)
+      atomicAdd(&acc[c], g);   // (a key listed twice counts twice; of three entries the order is not fixed)
       s_flags[c >> 7] = 1;
     }
   };
