@@ -309,6 +309,36 @@ def test_a_key_listed_twice_counts_twice():
         assert bool(((got.cpu().double() - want[name]).abs() <= err[name] + want[name].abs() * 2.0 ** -7 + 1e-30).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,S1,S2,N1,K", [(2, 5, 60, 7, 40), (1, 1501, 1280, 32, 1279)])
+def test_gradients_into_rows_of_any_alignment(B, S1, S2, N1, K, dtype):
+    """d_q of the C entry need only start at an element, queries without keys included; the elements around it stay as they are."""
+    from tilelang_ascend_b200 import _lib
+    g = torch.Generator().manual_seed(33)
+    query, key, weights, _ = (t.cuda() for t in make_indexer(g, B, S1, S2, N1, 4, dtype))
+    indices = torch.arange(K, dtype=torch.int32).expand(B, S1, 1, K).clone()
+    indices[0, 1], indices[-1, S1 - 1] = -1, -1
+    indices, d_values = indices.cuda(), torch.randn((B, S1, 1, K), generator=g).cuda()
+    sizes = B, S1, S2, N1, 128, K, _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_FP16
+    lib = _lib.load()
+    nbytes = lib.dsa_lightning_indexer_bwd_workspace_bytes(*sizes)
+    workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+    want = indexer_gradients(query.cpu(), key.cpu(), weights.cpu(), indices.cpu(), d_values.cpu())[0]["q"] if S1 < 100 else dsa.lightning_indexer_bwd_raw(
+        query, key, weights, indices, d_values)[0].cpu().double()
+    for offset in (1, 4):
+        buffer = torch.full((query.numel() + 8,), 7.0, dtype=dtype, device="cuda")
+        d_q = buffer[offset:offset + query.numel()].view(query.shape)
+        d_k, d_w = torch.zeros(key.shape, device="cuda"), torch.empty_like(weights)
+        _lib.check(lib.dsa_lightning_indexer_bwd(query.data_ptr(), key.data_ptr(), weights.data_ptr(), indices.data_ptr(), d_values.data_ptr(), d_q.data_ptr(),
+                                                 d_k.data_ptr(), d_w.data_ptr(), *sizes, workspace.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+        check_status()
+        # dz rounded once and the result once, on either side
+        assert relative(d_q, want) <= 4 * HALF_STEP[dtype]
+        assert not d_q[0, 1].any() and not d_q[-1, S1 - 1].any() and not d_w[0, 1].any()
+        assert bool((buffer[:offset] == 7).all()) and bool((buffer[offset + query.numel():] == 7).all())
+
+
 # ------------------------------------------------------------------------------------------------------ distillation
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,T", [("weights", 1.0), ("logits", 2.0)])

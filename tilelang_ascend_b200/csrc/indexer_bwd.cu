@@ -163,7 +163,11 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
       const float* w_row = p.w + static_cast<int64_t>(bt) * p.N1;
       if (!tiles) {
         T* dq = reinterpret_cast<T*>(p.d_q) + static_cast<int64_t>(bt) * p.N1 * kD;
-        for (int k = lane; k < p.N1 * kD / 8; k += 32) reinterpret_cast<uint4*>(dq)[k] = make_uint4(0, 0, 0, 0);
+        if ((reinterpret_cast<uintptr_t>(dq) & 15u) == 0) {
+          for (int k = lane; k < p.N1 * kD / 8; k += 32) reinterpret_cast<uint4*>(dq)[k] = make_uint4(0, 0, 0, 0);
+        } else {   // (d_q may start at any element)
+          for (int k = lane; k < p.N1 * kD; k += 32) dq[k] = static_cast<T>(0.f);
+        }
         for (int k = lane; k < p.N1; k += 32) p.d_w[static_cast<int64_t>(bt) * p.N1 + k] = 0.f;
         continue;
       }
