@@ -81,6 +81,49 @@ def test_key_weights(B, S, S_kv, H, D, K, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,S,S_kv,H,D,K", [
+    (1, 460, 700, 64, 576, 300),     # three to four queries in turn on every SM
+    (2, 301, 500, 128, 576, 257),
+    (1, 450, 600, 200, 576, 384),    # two passes over the heads
+    (1, 450, 500, 128, 640, 200),    # widest rows: three stages
+    (1, 1000, 1000, 24, 512, 130),   # causal from the first key on: lists of one tile and of two
+])
+def test_key_weights_of_more_queries_than_sms(B, S, S_kv, H, D, K, dtype):
+    """Queries that follow one another on an SM, queries without keys between them: against the definition on the GPU in 64 bits."""
+    g = torch.Generator().manual_seed(S + H)
+    q, kv = torch.randn((B, S, H, D), generator=g).to(dtype).cuda(), torch.randn((B, S_kv, 1, D), generator=g).to(dtype).cuda()
+    indices = lists(g, B, S, S_kv, K)
+    gone = torch.rand((B, S), generator=g) < 0.2
+    gone[:, S // 2:S // 2 + 3] = True
+    indices[gone] = -1
+    indices[-1, S - 9, 0, 128:] = -1          # a list that ends with its first tile
+    indices[-1, S - 8, 0, :128] = -1          # one that begins with its second
+    indices = indices.cuda()
+    lse = (torch.randn((B, S, H), generator=g) + 5).cuda()
+    lse[0, ::7, 1] = -INF
+    scale = 0.9 * D ** -0.5
+    got = dsa.sparse_mla_key_weights(q, kv, indices, lse, sm_scale=scale)
+    again = dsa.sparse_mla_key_weights(q, kv, indices, lse, sm_scale=scale)
+    check_status()
+    assert torch.equal(got, again)
+    last = torch.arange(S, device="cuda") + (S_kv - S)
+    for b in range(B):
+        for s0 in range(0, S, 50):
+            idx = indices[b, s0:s0 + 50, 0].long()
+            there = (idx >= 0) & (idx < S_kv) & (idx <= last[s0:s0 + 50, None])
+            rows, heads = kv[b, idx.clamp(0, S_kv - 1), 0].double(), q[b, s0:s0 + 50].double()
+            l = lse[b, s0:s0 + 50].double()[:, :, None]
+            w = torch.exp(heads @ rows.transpose(1, 2) * scale - torch.where(l == -INF, INF, l))
+            # (the bound of key_weights)
+            size = heads.abs() @ rows.abs().transpose(1, 2) * scale * (D / 16 + 1) * 2.0 ** -22 + (l.abs().nan_to_num(posinf=0) + 8) * 3 * 2.0 ** -24 + 2.0 ** -21
+            want = torch.where(there, w.mean(1), 0.0)
+            slack = torch.where(there, (w * size).mean(1) + w.mean(1) * H * 2.0 ** -24, 0.0)
+            err = (got[b, s0:s0 + 50, 0].double() - want).abs()
+            assert bool((err <= slack).all()), f"sequence {b}, queries from {s0}: off by {float((err - slack).max()):.3g}, largest weight {float(want.max()):.3g}"
+
+
+@pytest.mark.gpu
 def test_key_weights_are_the_forwards_softmax():
     """With the forward's own normalisers a list's weights add up to 1, and those of one head give its output."""
     g = torch.Generator().manual_seed(2)

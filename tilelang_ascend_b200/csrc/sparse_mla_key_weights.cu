@@ -260,7 +260,10 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
         bool full = false, room = g < 2;
         for (int i = 0; ok && i < count; ++i) {
           const int a = g & 1;
-          if (!room && !wait(&acc_free[a], ((g >> 1) + 1) & 1)) { ok = false; break; }
+          if (!room) {
+            if (!wait(&acc_free[a], ((g >> 1) + 1) & 1)) { ok = false; break; }
+            tc_fence_after();   // (the stage may have been seen, and fenced, before)
+          }
           const uint32_t acc = tmem + kColS + a * kKeys;
           room = g < 1;   // the tile after this one
           for (int part = 0; part < sh.parts; ++part) {
@@ -385,6 +388,7 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
             const int slot = list[i] * kKeys + tid;   // (of the combining threads, tid < 128)
             const int a = g & 1;
             ok = ok && __all_sync(0xffffffffu, mbar_wait<true>(&acc_full[a], (g >> 1) & 1, p.status));
+            tc_fence_after();   // ahead of the scores' loads and of the next heads' stores
             ring.skip(sh.parts, sh.stages);   // this tile's slots were the MMAs'
             if (i + 1 == count) {               // no MMA reads these heads any more: the next ones take their place before the epilogue
               if (pass + 1 < passes) {
@@ -400,7 +404,6 @@ __global__ void __launch_bounds__(kw::kThreads, 1)
                 }
               }
             }
-            tc_fence_after();
             // 32 keys at a time: this thread has two keys of every eight for four heads of its quarter, adds those up itself and ends, after
             // three halving exchanges with the lanes of the other heads, with the quarter's sum for one key.
             float* part = s_part + (a * 4 + quarter) * kKeys + half * 64;
