@@ -308,6 +308,70 @@ def test_gradient_of_one_side_alone():
     assert all(queries[i] is None for i in (1, 3, 4, 5)) and all(torch.equal(queries[i], both[i]) for i in (0, 2))
 
 
+def check_one_side(kind, B, S, H, D, R, start, n, interleaved, dtype, eps, seed):
+    """Output and gradients of queries alone against autograd through the definition (on the GPU, in 64 bits); upstream gradients above 0, so that rows
+    missing from the parameters' sums would show."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((B, S, H, D), generator=g).add(0.3).to(dtype).cuda()
+    d_out = torch.rand((B, S, H, D), generator=g).add(0.5).to(dtype).cuda()
+    weight, bias = (1 + 0.3 * torch.randn(n, generator=g)).cuda(), (0.2 * torch.randn(n, generator=g)).cuda() if kind == "layer" else None
+    positions = torch.randint(0, 50000, (B, S), generator=g).cuda()
+    inv_freq = (10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)).float().cuda()
+    names, leaves = (("x", "weight", "bias"), (x, weight, bias)) if bias is not None else (("x", "weight"), (x, weight))
+    mine = [t.detach().requires_grad_() for t in leaves]
+    out, _ = dsa.qk_norm_rope(mine[0], None, positions, inv_freq, rope_start=start, interleaved=interleaved, q_norm=kind, q_weight=mine[1],
+                              q_bias=mine[2] if bias is not None else None, norm_dim=n, eps=eps)
+    got = dict(zip(names, torch.autograd.grad(out, mine, d_out)))
+    exact = [t.double().requires_grad_() for t in leaves]
+    y = reference(exact[0], positions, inv_freq, kind, exact[1], exact[2] if bias is not None else None, n, start, interleaved, 1.0, eps)
+    want = dict(zip(names, torch.autograd.grad(y, exact, d_out.double())))
+    y = y.detach()
+    assert_rounded(out, y.cpu(), (ROW * 3 * y.abs().amax(-1, keepdim=True).clamp(min=1.0)).cpu(), "rows")
+    h = x.double()[..., :n]
+    h = h - h.mean(-1, keepdim=True) if kind == "layer" else h
+    rstd = (h.square().mean(-1, keepdim=True) + eps).rsqrt()
+    unit = h * rstd
+    most = unit.abs().amax(-1, keepdim=True).clamp(min=1.0)
+    u = rotate(d_out.double(), positions, inv_freq, start, interleaved, 1.0, back=True)
+    size = u.abs().amax(-1, keepdim=True) * (1 + rstd * (weight.double().abs().max() * 3 * most))
+    assert_rounded(got["x"], want["x"].cpu(), (2 * ROW * size).cpu(), "dx")
+    # sums over the rows: those of a block in turn at most (296 blocks), its groups, the blocks' lines.  A term u n is off by |u| times 2 ROW of the
+    # row's largest |n|, and by |n| times what u is off by: u = a cos + b sin with |a| + |b| <= 2 max|u| (a rotation of a pair of u), cosine and sine
+    # within 4 * 2^-24, two roundings: 12 * 2^-24 max|u| < ROW max|u|, however small u itself is
+    additions = (B * S * H / 296 + 128) * 2.0 ** -24
+    umax, u = ROW * u.abs().amax(-1, keepdim=True), u[..., :n].abs()
+    terms = additions * u * unit.abs() + 2 * ROW * u * most + umax * unit.abs()
+    assert_rounded(got["weight"], want["weight"].cpu(), terms.sum((0, 1, 2)).cpu(), "dweight")
+    if bias is not None:
+        assert_rounded(got["bias"], want["bias"].cpu(), (additions * u + umax).sum((0, 1, 2)).cpu(), "dbias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("B,S,H,D,R,start,n,interleaved", [
+    (1, 1, 1, 128, 64, 0, 128, False),     # one row
+    (2, 7, 3, 64, 64, 0, 64, True),        # rows that do not fill a block's groups
+    (1, 5, 1, 576, 64, 512, 512, True),
+    (1, 300, 3, 256, 64, 192, 192, False),
+    (1, 3, 2, 90, 30, 7, 61, True),        # element by element
+])
+def test_gradients_without_eps(B, S, H, D, R, start, n, interleaved, kind, dtype):
+    check_one_side(kind, B, S, H, D, R, start, n, interleaved, dtype, 0.0, seed=D + S)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,B,S,H,D,R,start,n,interleaved", [
+    ("rms", 2, 1201, 16, 128, 128, 0, 128, False),
+    ("layer", 1, 10007, 1, 576, 64, 512, 512, True),
+    ("layer", 3, 2003, 13, 64, 64, 0, 64, True),
+    ("rms", 1, 5003, 2, 90, 30, 7, 61, False),       # element by element
+])
+def test_parameter_gradients_over_more_rows_than_fit_the_chip(kind, B, S, H, D, R, start, n, interleaved):
+    """More tiles of rows than blocks: a block's sums go over several of them."""
+    check_one_side(kind, B, S, H, D, R, start, n, interleaved, torch.bfloat16, 1e-6, seed=D)
+
+
 # --------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_slots_and_of_a_side_alone():
     q, k = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)

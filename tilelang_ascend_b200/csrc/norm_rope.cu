@@ -366,7 +366,8 @@ __global__ void __launch_bounds__(nr::kThreads) norm_rope_bwd_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 8; ++j) { x[i][j] -= mean; q += x[i][j] * x[i][j]; }
         }
-      const float rstd = rsqrtf(group_sum<G>(q) * p.inv_norm_dim + p.eps);
+      const float square = group_sum<G>(q) * p.inv_norm_dim + p.eps;
+      const float rstd = live ? rsqrtf(square) : 0.f;   // (a group without a row holds zeros, and they stay zeros without an eps too)
       float gn = 0.f, gs = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
