@@ -382,6 +382,47 @@ def test_gradients_into_rows_of_any_alignment(B, S1, S2, N1, K, dtype):
         assert bool((buffer[:offset] == 7).all()) and bool((buffer[offset + query.numel():] == 7).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("level", [2.0 ** 8, 2.0 ** -60, 2.0 ** 90])
+def test_fp16_gradients_far_below_a_lists_largest(level):
+    """fp16: heads with small weights and keys with small gradients, 2^-22 of the list's largest, keep the digits of one rounding."""
+    g = torch.Generator().manual_seed(41)
+    B, S1, S2, N1, K = 1, 6, 300, 64, 200
+    query, key, _, indices = make_indexer(g, B, S1, S2, N1, K, torch.float16)
+    small_head, small_key = torch.arange(N1) % 2 == 1, torch.arange(S2) >= S2 // 2
+
+    def spread(shape):   # of either sign, from 1/2 to 1
+        return (0.5 + 0.5 * torch.rand(shape, generator=g)) * torch.where(torch.rand(shape, generator=g) < 0.5, -1.0, 1.0)
+
+    weights = spread((B, S1, N1)) * torch.where(small_head, 2.0 ** -22, 1.0)
+    d_values = spread(indices.shape) * torch.where(small_key[indices.clamp(0, S2 - 1).long()], 2.0 ** -22, 1.0)
+    if level < 1:
+        weights = weights * level          # (both factors far from 1, their product times the queries and keys inside fp16)
+        d_values = d_values * (2.0 ** 8 / level)
+    else:
+        weights = weights * (2.0 ** 8 / level)
+        d_values = d_values * level
+    dq, dk, dw = dsa.lightning_indexer_bwd_raw(query.cuda(), key.cuda(), weights.cuda(), indices.cuda(), d_values.cuda())
+    check_status()
+    want_q, want_k, err_q, err_k = (torch.zeros(t.shape, dtype=torch.float64) for t in (query, key, query, key))
+    for s in range(S1):
+        idx = indices[0, s, 0].long()
+        there = (idx >= 0) & (idx < S2)
+        idx, gr = idx[there], d_values[0, s, 0][there].double()
+        rows, heads, w = key[0, idx, 0].double(), query[0, s].double(), weights[0, s].double()
+        dz = torch.where(rows @ heads.T > 0, gr[:, None] * w, 0.0)
+        # a half step of fp16 (and of fp32 for its factors), half a step of its smallest values below 2^-27 of the largest; sums in fp32
+        top = float(gr.abs().max() * w.abs().max()) if gr.numel() else 0.0
+        off = dz.abs() * (2.0 ** -11 + 2.0 ** -16) + 2.0 ** -38 * top
+        want_q[0, s], err_q[0, s] = dz.T @ rows, off.T @ rows.abs()
+        want_k[0, :, 0].index_add_(0, idx, dz @ heads)
+        err_k[0, :, 0].index_add_(0, idx, off @ heads.abs())
+    off_q = (dq.cpu().double() - want_q).abs()
+    assert bool((off_q <= err_q + (want_q.abs() + err_q) * 2.0 ** -11 + 2.0 ** -25).all()), f"dq off, of small heads by {relative(dq[0, :, small_head.cuda()], want_q[0, :, small_head]):.3g}"
+    off_k = (dk.cpu().double() - want_k).abs()
+    assert bool((off_k <= err_k).all()), f"dk off, of small keys by {relative(dk[0, small_key.cuda()], want_k[0, small_key]):.3g}"
+
+
 # ------------------------------------------------------------------------------------------------------ distillation
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,T", [("weights", 1.0), ("logits", 2.0)])

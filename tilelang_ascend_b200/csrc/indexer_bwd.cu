@@ -16,7 +16,7 @@
 // (Two CTAs per SM whose warps made dZ and added in turn spent 8500 clocks on a tile, half of them without an addition on its way: 790 us;
 // one warp for all MMAs: 710.)
 // dz is rounded to the inputs' type (a tensor-core operand); its magnitude is that of the gradient, so fp16 takes it times a power
-// of two that brings the largest of a query's list near 1.  Sums are fp32.
+// of two that brings the largest of a query's list close under fp16's end.  Sums are fp32.
 #include <type_traits>
 
 #include "fwd_common.cuh"
@@ -38,8 +38,8 @@ constexpr int kUsers = kDzWarps + kAddWarps + kGatherWarps + 2;       // warps t
 struct List {
   int query;                 // b * S1 + s, -1: no more
   int tiles;                 // tiles with a key
-  float scale, unscale;      // of dz
-  float w[kHeads];
+  float scale, unscale;      // of a gradient; of the sums
+  float w[kHeads];           // scaled too
   uint32_t bits[kMaxWords];  // which entries take part
   uint8_t tile[kMaxTiles];   // the tiles with a key
 };
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
       const int32_t* idx_row = p.indices + static_cast<int64_t>(bt) * p.K;
       const float* g_row = p.grad + static_cast<int64_t>(bt) * p.K;
       int tiles = 0;
-      float top = 0.f;   // largest |g| of this lane's entries
+      float top = 0.f;   // largest finite |g| of this lane's entries
       for (int j0 = 0; j0 < p.K; j0 += 4 * kKeys) {   // four tiles' indices on their way at once
         int idx[16];
 #pragma unroll
@@ -151,7 +151,10 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
             const bool valid = idx[k] >= 0 && idx[k] < p.S2;
             const uint32_t bits = __ballot_sync(0xffffffffu, valid);
             if (lane == 0 && j0 + 32 * k < kMaxWords * 32) list.bits[j0 / 32 + k] = bits;
-            if (!kBF16 && valid) top = fmaxf(top, fabsf(__ldg(g_row + j0 + 32 * k + lane)));
+            if (!kBF16 && valid) {
+              const float size = fabsf(__ldg(g_row + j0 + 32 * k + lane));
+              if (size < INFINITY) top = fmaxf(top, size);
+            }
             any |= bits;
           }
           if (any) {
@@ -171,30 +174,33 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
         for (int k = lane; k < p.N1; k += 32) p.d_w[static_cast<int64_t>(bt) * p.N1 + k] = 0.f;
         continue;
       }
-      float top_w = 0.f;
+      float w[2], top_w = 0.f;   // (largest finite |w|)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int h = 32 * k + lane;
-        const float w = h < p.N1 ? __ldg(w_row + h) : 0.f;
-        list.w[h] = w;
-        top_w = fmaxf(top_w, fabsf(w));
+        w[k] = h < p.N1 ? __ldg(w_row + h) : 0.f;
+        if (fabsf(w[k]) < INFINITY) top_w = fmaxf(top_w, fabsf(w[k]));
       }
-      float scale = 1.f, unscale = 1.f;
+      float scale_w = 1.f, scale = 1.f, unscale = 1.f;
       if (!kBF16) {
-        // 2^-e with 2^e the exponent of max|g| max|w|: dz keeps fp16's range from the largest of the list downwards (what falls below
-        // 2^-24 of it is lost, as it is below fp32's last place of the sums)
+        // |dz| goes to 2^13 .. 2^15 at most, close under fp16's end: a head's or a key's sum need not hold the largest of the list, so all that lies
+        // below it counts.  A dz down to 2^-27 of the list's largest keeps fp16's 11 bits, what is smaller is off by 2^-38 of that largest.
+        // Gradients and weights take a power of two each, so that neither product leaves fp32.
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           top_w = fmaxf(top_w, __shfl_xor_sync(0xffffffffu, top_w, o));
         }
-        int e = 0;
-        if (top > 0.f && top < INFINITY) e += ilogbf(top);
-        if (top_w > 0.f && top_w < INFINITY) e += ilogbf(top_w);
-        e = max(-120, min(120, e));
-        scale = ldexpf(1.f, -e);
+        int eg = 0, ew = 0;
+        if (top > 0.f) eg = max(-113, ilogbf(top));
+        if (top_w > 0.f) ew = max(-126, min(126, ilogbf(top_w)));
+        const int e = max(-126, min(126, eg + ew - 13));
+        scale_w = ldexpf(1.f, -ew);
+        scale = ldexpf(1.f, ew - e);
         unscale = ldexpf(1.f, e);
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) list.w[32 * k + lane] = w[k] * scale_w;
       __syncwarp();
       if (lane == 0) {
         list.query = bt;
