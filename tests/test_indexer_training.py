@@ -423,6 +423,46 @@ def test_fp16_gradients_far_below_a_lists_largest(level):
     assert bool((off_k <= err_k).all()), f"dk off, of small keys by {relative(dk[0, small_key.cuda()], want_k[0, small_key]):.3g}"
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_that_are_not_finite_reach_the_gradients(dtype):
+    """NaN and infinities among listed queries and keys: NaN where autograd through the definition has them, the same values elsewhere; entries that take no
+    part stay out."""
+    g = torch.Generator().manual_seed(43)
+    B, S1, S2, N1, K = 1, 9, 300, 40, 150
+    query, key, weights, indices = make_indexer(g, B, S1, S2, N1, K, dtype)
+    clean = [t.clone() for t in (query, key)]
+    query[0, 2, 3, 5], query[0, 4, 6, 7] = float("nan"), INF
+    key[0, 7, 0, 9], key[0, 9, 0, 11] = float("nan"), -INF
+    indices[0, :, 0][(indices[0, :, 0] == 7) | (indices[0, :, 0] == 9)] = -1
+    indices[0, 6, 0, 100], indices[0, 7, 0, 20] = 7, 9      # one query lists each of them
+    d_values = torch.randn(indices.shape, generator=g)
+    d_values[indices < 0] = float("nan")
+    got = [t.cpu().double() for t in dsa.lightning_indexer_bwd_raw(query.cuda(), key.cuda(), weights.cuda(), indices.cuda(), d_values.cuda())]
+    check_status()
+
+    def definition(query, key):
+        leaves = [t.double().requires_grad_() for t in (query, key, weights)]
+        total = 0.0
+        for s in range(S1):
+            idx = indices[0, s, 0].long()
+            there = (idx >= 0) & (idx < S2)
+            scores = (leaves[1][0, idx[there], 0] @ leaves[0][0, s].T).relu() @ leaves[2][0, s]
+            total = total + (scores * d_values[0, s, 0][there].double()).sum()
+        return torch.autograd.grad(total, leaves)
+
+    want = definition(query, key)
+    sizes = definition(*clean)
+    for name, a, b, c in zip("qkw", got, want, sizes):
+        assert torch.equal(a.isnan(), b.isnan()), f"d{name}: {int(a.isnan().sum())} values are NaN, of {int(b.isnan().sum())}"
+        there = b.isfinite()
+        assert torch.equal(a[~there].nan_to_num(0.0), b[~there].nan_to_num(0.0)), f"d{name}: infinities"
+        # dz rounded once, the result once
+        off = float((a - b)[there].norm() / c.norm())
+        assert off <= 2 * HALF_STEP[dtype], f"d{name} off by {off:.3g} of its norm"
+    assert bool(want[2][0, 2, 3].isnan()) and bool(want[2][0, 6].isnan().all()) and int(want[2].isnan().sum()) < 3 * N1
+
+
 # ------------------------------------------------------------------------------------------------------ distillation
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,T", [("weights", 1.0), ("logits", 2.0)])

@@ -65,6 +65,12 @@ __device__ __forceinline__ bool bar_and(uint32_t id, uint32_t nthreads, bool yes
       : "memory");
   return all != 0;
 }
+// A NaN stays one, as in autograd's relu (whose gradient at NaN is that of a positive value).
+__device__ __forceinline__ float relu(float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
+}
 }  // namespace ib
 
 template <bool kBF16>
@@ -358,16 +364,16 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
       if (bt < 0) break;
       const float* g_row = p.grad + static_cast<int64_t>(bt) * p.K;
       const float scale = list.scale;
-      auto gradient = [&](int i) {   // of this thread's key of the list's tile number i
-        const int slot = list.tile[i] * kKeys + key;
-        return (list.bits[slot >> 5] >> lane) & 1u ? __ldg(g_row + slot) : 0.f;
-      };
+      // this thread's key of the list's tile number i: does it take part, and its gradient
+      auto takes_part = [&](int i) { return ((list.bits[list.tile[i] * (kKeys / 32) + quarter] >> lane) & 1u) != 0; };
+      auto gradient = [&](int i) { return takes_part(i) ? __ldg(g_row + list.tile[i] * kKeys + key) : 0.f; };
       float dw[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) dw[i] = 0.f;
       float next = gradient(0);
       for (int i = 0; i < list.tiles; ++i, ++g) {
         const float gr = next;
+        const bool there = takes_part(i);
         if (i + 1 < list.tiles) next = gradient(i + 1);
         ok = ok && wait(&z_full[g & 1], use(g));
         ok = ok && (g < 2 || wait(&dz_free[g & 1], before(g)));
@@ -380,6 +386,10 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
           uint32_t v[16], w[8];
           tmem_ld16(tmem_base + kColZ + (g & 1) * kHeads + half * 32 + c0 + lane_base, v);
           tmem_wait_ld();
+          if (!there) {   // (its row is zeros, but the query need not be finite)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = 0u;
+          }
           const float4* w4 = reinterpret_cast<const float4*>(list.w + half * 32 + c0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -388,12 +398,12 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               z[k] = __uint_as_float(v[4 * j + k]);
-              dw[c0 + 4 * j + k] = fmaf(gr, fmaxf(z[k], 0.f), dw[c0 + 4 * j + k]);
+              dw[c0 + 4 * j + k] = fmaf(gr, relu(z[k]), dw[c0 + 4 * j + k]);
             }
-            d[0] = z[0] > 0.f ? gs * wt.x : 0.f;
-            d[1] = z[1] > 0.f ? gs * wt.y : 0.f;
-            d[2] = z[2] > 0.f ? gs * wt.z : 0.f;
-            d[3] = z[3] > 0.f ? gs * wt.w : 0.f;
+            d[0] = z[0] <= 0.f ? 0.f : gs * wt.x;
+            d[1] = z[1] <= 0.f ? 0.f : gs * wt.y;
+            d[2] = z[2] <= 0.f ? 0.f : gs * wt.z;
+            d[3] = z[3] <= 0.f ? 0.f : gs * wt.w;
             w[2 * j] = pack2<kBF16>(d[0], d[1]);
             w[2 * j + 1] = pack2<kBF16>(d[2], d[3]);
           }

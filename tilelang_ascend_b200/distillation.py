@@ -175,8 +175,8 @@ def _check_indexer(query, key, weights, indices, lists) -> torch.device:
 
 def lightning_indexer_bwd_raw(query, key, weights, indices, d_values):
     """Gradients of the indexer's scores at listed keys: (d_query in the query's dtype, d_key fp32, d_weights fp32) for ``d_values``
-    [B,S1,1,K] fp32.  Entries of ``indices`` outside [0, S2) take no part, whatever d_values holds there.  relu'(0) = 0.  The key
-    gradient is summed with fp32 atomics: its last bits depend on their order (the others' only where a list names a key three times
+    [B,S1,1,K] fp32.  Entries of ``indices`` outside [0, S2) take no part, whatever d_values holds there.  relu'(0) = 0, and a score
+    that is NaN is passed on, as autograd's relu does.  The key gradient is summed with fp32 atomics: its last bits depend on their order (the others' only where a list names a key three times
     or more)."""
     _check_indexer(query, key, weights, indices, [(d_values, "d_values")])
     return _indexer_gradients(query, key, weights, indices, d_values)
