@@ -226,6 +226,25 @@ def test_repeatable_captured_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(first, other)) and all(torch.equal(a, b) for a, b in zip(captured, step()))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,K,over", [(300, None, "list"), (300, 40, "list"), (300, 40, "row"), (40000, 700, "row")])
+def test_a_teacher_whose_sum_is_not_finite(V, K, over):
+    """An infinite weight, or weights whose sum fp32 does not hold: NaN in the loss and in the gradient of the entries, other rows as they are."""
+    g, student, teacher, indices = rows(5, V, V if K is None else K, torch.float32, "weights", seed=V, listed=K is not None)
+    teacher[1, 2], teacher[3, :4] = INF, 3e38
+    if indices is not None:
+        indices[4, 5], teacher[4, 5] = -1, INF     # (takes no part)
+    else:
+        student[4, 5], teacher[4, 5] = -INF, INF
+    leaf = student.cuda().requires_grad_()
+    loss = dsa.topk_distillation(leaf, teacher.cuda(), None if indices is None else indices.cuda(), over=over)
+    (d,) = torch.autograd.grad(loss.sum(), leaf)
+    cols = torch.arange(V).repeat(5, 1) if indices is None else indices.long()
+    assert loss.isnan().tolist() == [False, True, False, True, False]
+    for r in range(5):
+        assert bool(d[r].cpu()[cols[r]].isnan().all()) == (r in (1, 3)) and (r in (1, 3) or bool(d[r].isfinite().all()))
+
+
 def test_refusals():
     s, t, i = torch.zeros(4, 10), torch.ones(4, 3), torch.zeros(4, 3, dtype=torch.int32)
     bad = [

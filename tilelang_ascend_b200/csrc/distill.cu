@@ -225,10 +225,11 @@ __device__ __forceinline__ void finish_row(const DistillParams& p, int64_t r, co
   const bool active = !(W == 0.f);   // (NaN: the loss says so)
   p.loss[r] = active ? sum[2] / W - logf(W) + logf(sum[0]) : 0.f;
   // for the backward: maximum and reciprocal sum of the student; of the teacher the maximum of the logits, or a factor that keeps
-  // the weights' reciprocal sum finite, and that reciprocal (0: no gradient)
+  // the weights' reciprocal sum finite, and that reciprocal (0: no gradient; an infinite sum has none: NaN, as the loss)
   const float factor = p.teacher_logits ? 1.f : (W < 0x1p-100f ? 0x1p100f : 1.f);
+  const float inv_W = W < INFINITY ? 1.f / (W * factor) : NAN;
   reinterpret_cast<float4*>(p.stats)[r] =
-      make_float4(top[0], active ? 1.f / sum[0] : 0.f, p.teacher_logits ? top[1] : factor, active ? 1.f / (W * factor) : 0.f);
+      make_float4(top[0], active ? 1.f / sum[0] : 0.f, p.teacher_logits ? top[1] : factor, active ? inv_W : 0.f);
 }
 
 // A block's kChunk columns in registers: 16-byte units (kWide) or single elements, kListedThreads apart.

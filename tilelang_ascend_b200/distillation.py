@@ -144,7 +144,7 @@ def topk_distillation(student, teacher, indices: Optional[torch.Tensor] = None, 
     """KL divergence, row by row, of a student's logits from a teacher's top entries: ``loss = sum_j p_j (log p_j - log s_j)``.
 
     student [..., V] fp32 / bf16 / fp16 logits (unit inner stride, evenly spaced rows); teacher [..., K] the entries' ``"weights"``
-    (not below 0, any sum) or ``"logits"``; indices [..., K] int32 their columns, or None when every column has its entry (K = V).
+    (not below 0, any sum that fp32 holds; beyond, the row's loss is NaN) or ``"logits"``; indices [..., K] int32 their columns, or None when every column has its entry (K = V).
     An entry takes part when its column lies in [0, V) and the student's logit there is not -inf; -1 pads a list, and what the
     teacher holds at entries that take no part is not looked at.  p are the participating entries normalised (logits: softmax of
     logit / temperature), s the softmax of student / temperature ``over`` the participating entries (``"list"``) or over the whole row
@@ -176,8 +176,8 @@ def _check_indexer(query, key, weights, indices, lists) -> torch.device:
 def lightning_indexer_bwd_raw(query, key, weights, indices, d_values):
     """Gradients of the indexer's scores at listed keys: (d_query in the query's dtype, d_key fp32, d_weights fp32) for ``d_values``
     [B,S1,1,K] fp32.  Entries of ``indices`` outside [0, S2) take no part, whatever d_values holds there.  relu'(0) = 0, and a score
-    that is NaN is passed on, as autograd's relu does.  The key gradient is summed with fp32 atomics: its last bits depend on their order (the others' only where a list names a key three times
-    or more)."""
+    that is NaN is passed on, as autograd's relu does.  The key gradient is summed with fp32 atomics: its last bits depend on their
+    order (the others' only where a list names a key three times or more)."""
     _check_indexer(query, key, weights, indices, [(d_values, "d_values")])
     return _indexer_gradients(query, key, weights, indices, d_values)
 
