@@ -324,7 +324,7 @@ typedef struct dsa_rope_grads {
   void* d_bias;
 } dsa_rope_grads;
 
-/* Backward of dsa_norm_rope.  workspace: dsa_norm_rope_bwd_workspace_bytes(norm_dim) for each of q and k that asks for d_weight or
+/* Backward of dsa_norm_rope.  workspace (4-byte aligned): dsa_norm_rope_bwd_workspace_bytes(norm_dim) for each of q and k that asks for d_weight or
  * d_bias.  Those sums are taken in a fixed order. */
 size_t dsa_norm_rope_bwd_workspace_bytes(int32_t norm_dim);
 int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const void* positions, int32_t positions_int64, const float* inv_freq,
@@ -336,7 +336,7 @@ int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const vo
  * [0, V) and the student's logit there is not -inf; p = the teacher's entries (weights, or exp(logit / temperature) when
  * teacher_logits) over their sum, s = softmax(student / temperature) over the participating entries, or over the whole row when
  * over_row: loss [rows] fp32 = sum p (log p - log s), 0 for rows without teacher weight.  stats [rows, 4] fp32 (16-byte aligned) is
- * what the backward needs.  workspace: dsa_topk_distillation_workspace_bytes (0: NULL).  dtypes: 0 bfloat16, 1 float16, 2 float32.
+ * what the backward needs.  workspace (4-byte aligned): dsa_topk_distillation_workspace_bytes (0: NULL).  dtypes: 0 bfloat16, 1 float16, 2 float32.
  * No reference counterpart. */
 size_t dsa_topk_distillation_workspace_bytes(int64_t rows, int32_t V, int32_t over_row, int32_t listed);
 int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t row_stride, const void* teacher, int32_t teacher_dtype,

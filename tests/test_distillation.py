@@ -280,3 +280,14 @@ def test_c_entry_refuses_before_any_cuda_call():
     lib = _lib.load()
     assert lib.dsa_topk_distillation(None, 2, 4, None, 2, None, None, None, 1, 4, 4, 0, 0, 1.0, None, 0, None) != 0
     assert lib.dsa_topk_distillation_bwd(None, 2, 4, None, 2, None, None, None, None, 1, 4, 4, 0, 0, 1.0, None) != 0
+
+
+def test_c_entry_refuses_a_workspace_off_its_alignment():
+    from tilelang_ascend_b200 import _lib
+    lib = _lib.load()
+    rows, V, K = 3, 40000, 5
+    nbytes = lib.dsa_topk_distillation_workspace_bytes(rows, V, 1, 1)
+    assert nbytes > 0
+    at = 4096   # (an address that nothing reads: the call is refused before any launch)
+    assert lib.dsa_topk_distillation(at, 2, V, at, 2, at, at, at, rows, V, K, 1, 0, 1.0, at + 2, nbytes, None) != 0
+    assert b"aligned" in lib.dsa_get_last_error()

@@ -433,3 +433,14 @@ def test_c_entry_refuses_before_any_cuda_call():
     scalars = (None, 0, None, 1, 1, 64, 32, 0, 0, 1, 1.0, 1e-6)
     assert lib.dsa_norm_rope(None, None, *scalars, 0, None) != 0 and b"given" in lib.dsa_get_last_error()
     assert lib.dsa_norm_rope_bwd(None, None, *scalars, None, 0, 0, None) != 0
+
+
+def test_c_entry_refuses_a_workspace_off_its_alignment():
+    from ctypes import byref
+    from tilelang_ascend_b200 import _lib
+    lib = _lib.load()
+    at = 4096   # (an address that nothing reads: the call is refused before any launch)
+    rows = _lib.RopeRows(at, 64, 64, 64, 1, 1, at, None, 1, 64, at, None, None, 0, 0, 0)
+    side = _lib.RopeGrads(rows, at, 64, 64, 64, at, None)
+    assert lib.dsa_norm_rope_bwd(byref(side), None, at, 0, at, 1, 1, 64, 32, 0, 64, 1, 1.0, 1e-6, at + 1, 1 << 30, 0, None) != 0
+    assert b"aligned" in lib.dsa_get_last_error()

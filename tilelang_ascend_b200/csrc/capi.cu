@@ -624,6 +624,7 @@ int dsa_norm_rope_bwd(const dsa_rope_grads* q, const dsa_rope_grads* k, const vo
       if (!g->rows.norm) return fail("gradients of norm parameters need a norm");
       const size_t need = dsa::norm_rope_bwd_workspace_bytes(norm_dim);
       if (!workspace || workspace_bytes < used + need) return fail("workspace too small (see dsa_norm_rope_bwd_workspace_bytes)");
+      if (reinterpret_cast<uintptr_t>(workspace) & 3u) return fail("workspace must be 4-byte aligned");
       p.side[i].partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + used);
       used += need;
     }
@@ -647,6 +648,7 @@ int dsa_topk_distillation(const void* student, int32_t student_dtype, int64_t ro
   p.loss = loss;
   const size_t need = dsa::distill_workspace_bytes(rows, V, over_row, indices != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return fail("workspace too small (see dsa_topk_distillation_workspace_bytes)");
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 3u)) return fail("workspace must be 4-byte aligned");
   p.partials = need ? static_cast<float*>(workspace) : nullptr;
   int err = dsa::launch_distill_fwd(p, static_cast<cudaStream_t>(stream));
   return err ? fail_cuda("topk_distillation launch", err) : 0;
