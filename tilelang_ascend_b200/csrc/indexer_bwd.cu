@@ -142,12 +142,14 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
       const float* g_row = p.grad + static_cast<int64_t>(bt) * p.K;
       int tiles = 0;
       float top = 0.f;   // largest finite |g| of this lane's entries
-      for (int j0 = 0; j0 < p.K; j0 += 4 * kKeys) {   // four tiles' indices on their way at once
+      for (int j0 = 0; j0 < p.K; j0 += 4 * kKeys) {   // four tiles' entries on their way at once
         int idx[16];
+        float size[16];   // (fp16)
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int j = j0 + 32 * k + lane;
           idx[k] = j < p.K ? __ldg(idx_row + j) : -1;
+          if (!kBF16) size[k] = j < p.K ? fabsf(__ldg(g_row + j)) : 0.f;
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -157,10 +159,7 @@ __global__ void __launch_bounds__(ib::kThreads, 1) indexer_bwd_kernel(const __gr
             const bool valid = idx[k] >= 0 && idx[k] < p.S2;
             const uint32_t bits = __ballot_sync(0xffffffffu, valid);
             if (lane == 0 && j0 + 32 * k < kMaxWords * 32) list.bits[j0 / 32 + k] = bits;
-            if (!kBF16 && valid) {
-              const float size = fabsf(__ldg(g_row + j0 + 32 * k + lane));
-              if (size < INFINITY) top = fmaxf(top, size);
-            }
+            if (!kBF16) top = fmaxf(top, valid && size[k] < INFINITY ? size[k] : 0.f);
             any |= bits;
           }
           if (any) {
