@@ -52,19 +52,6 @@ constexpr uint32_t kSmemBytes = kOffList + 2 * sizeof(List);
 constexpr uint32_t kColZ = 0, kColDq = 128, kColDk = 256, kTmemCols = 512;   // two of each: 64, 64 and 128 columns
 static_assert(kSmemBytes <= 232448 && sizeof(List) % 16 == 0, "shared memory per CTA");
 
-// Barrier over nthreads threads that tells all of them whether all of them say yes.
-__device__ __forceinline__ bool bar_and(uint32_t id, uint32_t nthreads, bool yes) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(yes ? 1u : 0u), "r"(id), "r"(nthreads)
-      : "memory");
-  return all != 0;
-}
 // A NaN stays one, as in autograd's relu (whose gradient at NaN is that of a positive value).
 __device__ __forceinline__ float relu(float z) {
   float r;

@@ -26,20 +26,6 @@
 namespace dsa {
 
 namespace kw {
-// Barrier over nthreads threads that tells all of them whether all of them say yes.
-__device__ __forceinline__ bool bar_and(uint32_t id, uint32_t nthreads, bool yes) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(yes ? 1u : 0u), "r"(id), "r"(nthreads)
-      : "memory");
-  return all != 0;
-}
-
 constexpr int kKeys = 128;                        // keys per tile = UMMA N
 constexpr int kHeads = 128;                       // heads per pass over the list = UMMA M
 constexpr uint32_t kChunkBytes = 128 * 128;       // 128 keys (or heads) x 64 dims
