@@ -359,8 +359,9 @@ int dsa_sparse_mla_key_weights(const void* q, const void* kv, const int32_t* ind
 
 /* Backward of the indexer's scores at listed keys: q [B, S1, N1, 128], k [B, S2, 1, 128], w [B, S1, N1] fp32, indices [B, S1, 1, K]
  * (entries outside [0, S2) take no part), grad [B, S1, 1, K] fp32 of the scores there.  d_q (inputs' type) and d_w (fp32) are
- * written, d_k [B, S2, 1, 128] fp32 is added to (the order of its additions is not fixed, nor that of three or more entries of one key in d_q and d_w).  N1 at most 64, K at most 8192; q and k
- * 16-byte aligned, the others to their elements.  relu'(0) = 0.  workspace (16-byte aligned): dsa_lightning_indexer_bwd_workspace_bytes (0: NULL).  No reference counterpart. */
+ * written, d_k [B, S2, 1, 128] fp32 is added to (the order of its additions is not fixed, nor that of three or more entries of one key
+ * in d_q and d_w).  N1 at most 64, K at most 8192; q and k 16-byte aligned, the others to their elements.  relu'(0) = 0, relu(NaN) = NaN.
+ * workspace (16-byte aligned): dsa_lightning_indexer_bwd_workspace_bytes (0: NULL; about 1 GiB at most).  No reference counterpart. */
 size_t dsa_lightning_indexer_bwd_workspace_bytes(int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype);
 int dsa_lightning_indexer_bwd(const void* q, const void* k, const float* w, const int32_t* indices, const float* grad, void* d_q, float* d_k,
                               float* d_w, int32_t B, int32_t S1, int32_t S2, int32_t N1, int32_t D, int32_t K, int32_t dtype, void* workspace,

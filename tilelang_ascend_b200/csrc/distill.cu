@@ -341,6 +341,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) distill_fwd_kernel(const __
 // forward of wide rows, in parts: block = (row, kPartChunks chunks of its columns).  A chunk passes through one of two shared-memory
 // buffers, the next one on its way meanwhile, and the listed entries of its columns are looked up there: gathered from global memory,
 // 2048 entries of a row of 131072 cost as much as half of the row (1024 such rows: 141 us; one chunk per block: 147 us).
+// A thread holds the first 2048 entries' columns; what a list has behind them is read again for every chunk.  In parts / a row per block, fp32,
+// out of HBM, us: 1024 rows of 131072: 64 entries 104 / 107, 2048: 119 / 156, 4096: 168 / 205, 16384: 440 / 459, 65536: 1516 / 1409; 4 such
+// rows: 2048: 16 / 18, 4096: 21 / 18, 16384: 51 / 25; 1024 rows of 20000: 64: 35 / 27, 2048: 47 / 41, 8192: 102 / 68.  So parts are taken for their gain on
+// many wide rows with lists up to 16384, and lose on rows of a few parts and on few rows with long lists.
 // kWide: rows in aligned 16-byte units, copied asynchronously; else element by element.
 // -------------------------------------------------------------------------------------------------
 template <typename T, bool kWide>

@@ -12,7 +12,7 @@
 // dK^T has a dim per lane, so a warp adds 32 consecutive dims of a key to the fp32 gradient with one 128-byte request; these additions
 // (512 bytes per pair of query and key) are what bounds the kernel.  So everything else is kept out of their way: eight warps do
 // nothing else, eight others make dZ, four gather, one issues Z's MMAs and one the sums', one reads the next query's list; Z, dZ, dK^T and
-// dQ^T exist twice.  Measured for 4096 queries x 2048 of 4096 keys, 64 heads (3.2 GB of additions): 670 us, 4.8 TB/s; without the additions 478.
+// dQ^T exist twice.  Measured for 4096 queries x 2048 of 4096 keys, 64 heads (3.2 GB of additions): 674 us, 4.8 TB/s; without the additions 478; fp16 698.
 // (Two CTAs per SM whose warps made dZ and added in turn spent 8500 clocks on a tile, half of them without an addition on its way: 790 us;
 // one warp for all MMAs: 710.)
 // dz is rounded to the inputs' type (a tensor-core operand); its magnitude is that of the gradient, so fp16 takes it times a power

@@ -565,8 +565,8 @@ int launch_both(const IndexerBwdParams& p, const ibd::Dense& d, const CUtensorMa
 // Which kernel: the other one takes about 100 ps per (query, listed key), whatever the heads; these take 8 ps per (query, key that it may see) for
 // G, 42 more with 64 heads, half and a quarter of that with 32 and 16, and 30 us for three more launches.  Both counts as they are
 // in a causal step (keys up to S2 - S1 + t) with full lists.  Measured, other / these, us (queries x keys, list): 64 heads: 4096 x 4096, 2048:
-// 670 / 469, 1024: 412 / 459; 4096 x 8192, 2048: 855 / 1206; 1024 x 4096, 2048: 224 / 238; 32 heads: 2048 x 2048, 2048: 251 / 120; 4096 x 8192,
-// 2048: 850 / 677; 16 heads: 4096 x 4096, 512: 254 / 195; 4096 x 1024, 512: 262 / 122.  fp16 stays with the other kernel: its range needs a
+// 674 / 459, 1024: 416 / 459; 4096 x 8192, 2048: 862 / 1206; 1024 x 4096, 2048: 233 / 238; 32 heads: 2048 x 2048, 2048: 258 / 119; 4096 x 8192,
+// 2048: 854 / 625; 16 heads: 4096 x 4096, 512: 260 / 184; 4096 x 1024, 512: 262 / 122.  fp16 stays with the other kernel: its range needs a
 // scale per query.
 static bool dense_preferred(const IndexerBwdParams& p, bool bf16) {
   if (!bf16 || p.D != ibd::kD || (p.N1 != 16 && p.N1 != 32 && p.N1 != 64)) return false;

@@ -589,9 +589,9 @@ void tile(NormRopeParams* p, int which, int rows) {
   sd.tile_tokens = tokens < 1 ? 1 : tokens;
   sd.blocks = ((p->tokens + sd.tile_tokens - 1) / sd.tile_tokens) * ((sd.H + sd.tile_heads - 1) / sd.tile_heads);
 }
-// Rows per block: about 32 KB of them, which amortises a block's angles and weights (4096 tokens, rows of 576 dims: 32 rows 194 us, 128 rows
-// 198; rows of 128 dims, forward + backward: 32 rows 115 us, 128 rows 103); calls whose blocks all fit the chip at once (three per SM) take
-// shorter ones as long as they do (64 tokens x 129 rows of 576 dims: 32 rows 10.4 us, 16 rows -- more blocks than fit -- 14.4).
+// Rows per block: about 32 KB of them, which amortises a block's angles and weights (when the prefill call above took 194 us with 32 rows of
+// 576 dims, 128 rows took 198; rows of 128 dims, forward + backward, 115 us with 32 rows, 103 with 128); calls whose blocks all fit the
+// chip at once (three per SM) take shorter ones as long as they do (64 tokens x 129 rows of 576 dims: 32 rows 10.4 us, 16 rows -- more blocks than fit -- 14.4).
 void tiles(NormRopeParams* p, int sms) {
   int rows = 256;
   while (rows > 32 && rows * p->D > 16384) rows >>= 1;

@@ -16,6 +16,8 @@
 // Shuffles, copies and barriers share one pipe, so the sum over heads uses few: a thread takes four heads of the same keys out of
 // tensor memory and seven shuffles join 32 keys over a warp (one head per thread: 31; with that the epilogue took 3600 of the 2304
 // clocks that a tile's MMAs take, and the copies waited behind it: 848 us).
+// The exponentials are the hardware's ex2.approx of fp32 arguments: the weights are within 6e-7 of the definition (1e-7 with an exact
+// exponential), far inside what bf16 or fp16 queries and keys carry.
 // Measured there: 812 us, 1140 TFLOP/s.  A tile takes about 3200 clocks and a change of queries about 6000; what shares the tile's time is shared
 // memory: without the copies 650 us, without the epilogue 755.
 #include <type_traits>

@@ -144,7 +144,8 @@ def topk_distillation(student, teacher, indices: Optional[torch.Tensor] = None, 
     """KL divergence, row by row, of a student's logits from a teacher's top entries: ``loss = sum_j p_j (log p_j - log s_j)``.
 
     student [..., V] fp32 / bf16 / fp16 logits (unit inner stride, evenly spaced rows); teacher [..., K] the entries' ``"weights"``
-    (not below 0, any sum that fp32 holds; beyond, the row's loss is NaN) or ``"logits"``; indices [..., K] int32 their columns, or None when every column has its entry (K = V).
+    (not below 0, any sum from 1e-30 to 3e38; what fp32 cannot add up gives NaN) or ``"logits"``; indices [..., K] int32 their columns,
+    or None when every column has its entry (K = V).
     An entry takes part when its column lies in [0, V) and the student's logit there is not -inf; -1 pads a list, and what the
     teacher holds at entries that take no part is not looked at.  p are the participating entries normalised (logits: softmax of
     logit / temperature), s the softmax of student / temperature ``over`` the participating entries (``"list"``) or over the whole row

@@ -220,7 +220,7 @@ def qk_norm_rope_cached(q, k, positions, inv_freq, key_cache, slots, *, key_cach
     key_cache [num_blocks, block_size, Hk, D], or with ``key_cache_rope`` [num_blocks, block_size, Hk, R] the dims before the
     rotated ones, [num_blocks, block_size, Hk, D - R] (then the rotated dims are the last R).  slots [B,S] int32 / int64: block *
     block_size + offset; a token whose slot lies outside the cache (-1: padding) writes nothing.  Two tokens of a call never
-    share a slot.  One launch; no gradients (an input that asks for one is refused)."""
+    share a slot, and q and k are no part of the cache.  One launch; no gradients (an input that asks for one is refused)."""
     if k is None:
         raise ValueError("k must be given")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, q_bias, k_weight, k_bias)):
